@@ -72,7 +72,8 @@ uint64_t nntr_cuda_launch_count(void);
  *  gave up on one of its bounded waits (every device-side wait has an iteration
  *  limit; on expiry the kernel raises a status word and returns instead of
  *  hanging): NNTR_CUDA_OK, or NNTR_CUDA_ERR_TIMEOUT. NNTR_CUDA_ERR_INVALID: a
- *  kernel found an expert's weights that are not 16-byte aligned in a table. */
+ *  kernel found an expert's weights that are not 16-byte aligned in a table, or a
+ *  paged call's arrays contradict its bounds. */
 int nntr_cuda_device_status(void);
 /** Zeroes every status word of the bound device, so that a process that has seen NNTR_CUDA_ERR_TIMEOUT (or a
  *  rejected embedding index) can go on: nntr_cuda_device_status() reports a condition once per occurrence only if
@@ -337,11 +338,83 @@ int nntr_cuda_attention_rows_dev(const nntr_attn_desc *a, unsigned pos, unsigned
                                  float eps, void *kcache, void *vcache, const float *cos_tab, const float *sin_tab, float *out,
                                  size_t ld_out, unsigned flags, void *stream);
 
+/* ------------------------------------------- several sequences, a cache in pages */
+
+#define NNTR_F32 0
+#define NNTR_F16 1
+#define NNTR_BF16 30
+
+/** One layer's key/value cache in pages, which many sequences share: page p of either cache begins p * page_stride elements behind
+ *  its pointer and holds page_size rows of [kv head][head_dim], as a row of the contiguous caches above. Device pointers,
+ *  16-byte aligned; page_stride 0 = pages back to back, else a multiple of 8. dtype NNTR_F16 or NNTR_BF16; page_size 16, 32, 64, 128 or
+ *  256; head_dim a multiple of 8 of at most 128; n_heads_q a multiple of n_heads_kv. */
+typedef struct {
+  unsigned n_heads_q, n_heads_kv, head_dim;
+  int dtype;
+  unsigned page_size, n_pages;
+  int64_t page_stride;
+  void *kcache, *vcache;
+} nntr_paged_cache;
+/** The new tokens of a batch of sequences. Sequence b has the query rows row_start[b] .. row_start[b + 1] - 1, the last of
+ *  the context[b] rows that it has in the cache with them: query i is at position context[b] - new + i. Row r of the sequence lies
+ *  in page page_table[b * ld_table + r / page_size], which other sequences may share. The arrays are device memory, so that a
+ *  captured graph can be replayed with other contents; the numbers beside them are host-side bounds: `tokens` rows that q and the
+ *  results hold, no more than max_new rows of one sequence, contexts of about max_rows (0: not known; it chooses how the work is split,
+ *  any context is right). Rows of q and of the results behind the last sequence are neither read nor written.
+ *  Arrays that contradict the bounds or themselves (more rows than max_new, a context of fewer rows than the sequence has new ones,
+ *  rows behind the page table, a page outside the pool that is needed) touch no memory out of range: rows of such a page read as zeros
+ *  and are not stored, queries in front of position 0 see nothing, rows beyond the bounds are left as they were, and
+ *  nntr_cuda_device_status() returns NNTR_CUDA_ERR_INVALID. */
+typedef struct {
+  unsigned batch, tokens, max_new, max_rows, ld_table;
+  const int *row_start;  /* [batch + 1] */
+  const int *context;    /* [batch] */
+  const int *page_table; /* [batch][ld_table] */
+} nntr_paged_batch;
+/** The new tokens' rows of all sequences into the pages, in one pass: per-head RMS norms of q and k times q_gamma / k_gamma
+ *  [head_dim] (both or neither), rotary embedding by row `position` of cos_tab / sin_tab (DEVICE fp32 [table_rows][head_dim], as
+ *  nntr_cuda_rope_table fills them), k and v rounded into the caches, q rounded to the caches' type into q_out: what
+ *  nntr_cuda_qk_norm_rope_cache_append_dev does for one token of one sequence, with sums in another order. q, k, v: fp32 rows
+ *  ld_q, ld_kv, ld_kv elements apart (slices of one projection's output); q_out: rows ld_out elements apart (a multiple of 4, 8-byte
+ *  aligned). A token whose position has no row in the tables is not stored, its query is zero, and nntr_cuda_device_status() tells. A row
+ *  of a page that two sequences share must be new to one of them only. */
+int nntr_cuda_paged_append_dev(const nntr_paged_cache *c, const nntr_paged_batch *b, const float *q, const float *k, const float *v,
+                               int64_t ld_q, int64_t ld_kv, const float *q_gamma, const float *k_gamma, float eps,
+                               const float *cos_tab, const float *sin_tab, unsigned table_rows, void *q_out, int64_t ld_out,
+                               unsigned flags, void *stream);
+/** Attention of the new tokens over the pages (their own rows are in them already). The query at position p sees the rows
+ *  j <= p with j > p - window (UINT_MAX: all) or j < first_tokens; scores are scaled by 1 / sqrt(head_dim); sink: device fp32 [n_heads_q]
+ *  logits that join the softmax without a value, or NULL. A query that sees nothing gets zeros. Cache rows that no query of a sequence sees may
+ *  hold anything; the rows that one of them sees are expected to be finite. q: rows of the caches' type; out: of the same type
+ *  or fp32 (out_dtype NNTR_F32); both 16-byte aligned, ld_q and ld_out multiples of 8. Scores, sums and accumulators are fp32,
+ *  probabilities are rounded to the caches' type before they meet the values: the difference from exact arithmetic is about one
+ *  rounding to that type (also of fp32 results). No workspace. Not bit-compatible with nntr_cuda_attention_step_dev. */
+int nntr_cuda_paged_attention_dev(const nntr_paged_cache *c, const nntr_paged_batch *b, const void *q, int64_t ld_q,
+                                  unsigned window, unsigned first_tokens, const float *sink, void *out, int out_dtype,
+                                  int64_t ld_out, unsigned flags, void *stream);
+/** Copies whole pages: page src[i] -> page dst[i] for i < n, in each of `arrays` arrays of n_pages pages of page_bytes bytes
+ *  (a multiple of 16) that begin array_bytes apart (the key and value caches of all layers), in one launch. src and dst are device
+ *  arrays; no page may be in dst twice, or in both src and dst. Pairs with a page outside the pool are left out, and
+ *  nntr_cuda_device_status() returns NNTR_CUDA_ERR_INVALID. */
+int nntr_cuda_copy_pages_dev(void *base, unsigned arrays, int64_t array_bytes, int64_t page_bytes, unsigned n_pages, const int *src,
+                             const int *dst, unsigned n, unsigned flags, void *stream);
+/** A token per row of n logits (row stride ld), from the random number u[row] in [0, 1) (device): with weights
+ *  w = exp((x - max) / temperature) and tokens in descending order of x (the lowest index first among equals), top_k (0: off) keeps the
+ *  first ones, top_p (1: off) of these the shortest prefix whose weights reach top_p of their sum, min_p (0: off) of these the ones with
+ *  w >= min_p; the token is the first kept one in ascending order of the index up to which the kept weights exceed u times their sum.
+ *  temperature 0 or top_p 0: the greatest logit, as nntr_cuda_argmax_dev. -inf and NaN are never drawn; a row of nothing else gives 0.
+ *  row_params: device [rows][4] of (temperature, top_k, top_p, min_p) for each row in place of the four numbers, or NULL; there a
+ *  temperature or top_p that is not above 0 means the greatest logit.
+ *  idx_out (uint32) and / or idx_out_f (as a float) may be NULL; prob_out, or NULL: the token's weight over the kept ones' sum.
+ *  Weights are double precision, sums are exact: the token does not depend on how the work is split. Up to 2^20 logits,
+ *  65535 rows. */
+int nntr_cuda_sample_dev(const float *logits, int64_t rows, int64_t n, int64_t ld, const float *u, double temperature, unsigned top_k,
+                         double top_p, double min_p, const float *row_params, unsigned *idx_out, float *idx_out_f, float *prob_out,
+                         unsigned flags, void *stream);
+
 /* ------------------------------------------------------- .bin weight files */
 
 /** One tensor of a model file, in the order the model's layers request their weights. */
-#define NNTR_F32 0
-#define NNTR_F16 1
 typedef struct {
   int dtype;     /* NNTR_F32, NNTR_F16, NNTR_Q4_0, NNTR_Q4_K or NNTR_Q6_K */
   unsigned N, K; /* quantized: N rows of K weights (the tensor's width x height); fp: N * K elements */

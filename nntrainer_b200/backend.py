@@ -575,6 +575,266 @@ class Attention:
         return out
 
 
+# ------------------------------------------- several sequences, a cache in pages
+def _on_device(*tensors) -> None:
+    """Kernels are launched on the current device, whose stream they are put into: the tensors have to lie there."""
+    here = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("a CUDA tensor is needed (there is no CPU path)")
+        if here is None:
+            here = _torch()._C._cuda_getDevice()
+        if t.get_device() != here:
+            raise ValueError(f"a tensor on cuda:{t.get_device()}, the current device is cuda:{here}")
+
+
+def _typed(t, name: str, dtype, numel: int | None = None):
+    """A dense array of that type; its address. None passes."""
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        raise ValueError(f"{name}: need a contiguous {dtype} tensor" + (f" of {numel} elements" if numel is not None else ""))
+    return t.data_ptr()
+
+
+def _paged(kcache, vcache, n_heads_q: int, page_table, row_start, context, tokens: int, max_new: int, max_rows: int):
+    """The structures of a paged call from its tensors."""
+    torch = _torch()
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != vcache.dtype or kcache.stride() != vcache.stride():
+        raise ValueError("kcache and vcache: [n_pages, page_size, n_heads_kv, head_dim], alike in type and strides")
+    pages, ps, hkv, hd = kcache.shape
+    stride = kcache.stride()
+    if stride[3] != 1 or stride[2] != hd or stride[1] != hkv * hd:
+        raise ValueError("kcache and vcache: the rows of a page lie back to back")
+    dtype = {torch.float16: capi.F16, torch.bfloat16: capi.BF16}.get(kcache.dtype)
+    if dtype is None:
+        raise NotImplementedError(f"caches of fp16 or bf16 (got {kcache.dtype})")
+    batch = context.numel()
+    if page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise ValueError("page_table: [batch, pages of a sequence]")
+    c = capi.PagedCache(n_heads_q, hkv, hd, dtype, ps, pages, stride[0] if pages > 1 else 0, kcache.data_ptr(), vcache.data_ptr())
+    b = capi.PagedBatch(batch, tokens, max_new, max_rows, page_table.shape[1], _typed(row_start, "row_start", torch.int32, batch + 1),
+                        _typed(context, "context", torch.int32), _typed(page_table, "page_table", torch.int32))
+    from ctypes import byref
+    return byref(c), byref(b), dtype
+
+
+def paged_append(q, k, v, kcache, vcache, page_table, row_start, context, max_new: int, cos, sin, qk_norm=None, q_out=None,
+                 pdl: bool = False):
+    """The new tokens of a batch of sequences into a cache in pages, in one pass: per-head RMS norms of q and k (``qk_norm`` =
+    (q_gamma, k_gamma, eps)), rotary embedding, k and v rounded into the pages. Returns the rotated queries in the caches' type,
+    [tokens, n_heads_q, head_dim]. q [tokens, n_heads_q * head_dim], k and v [tokens, n_heads_kv * head_dim]: fp32, rows may be slices of
+    wider ones; cos, sin: device tables as ``rope_table`` makes them. The arrays of the batch: see ``paged_attention``."""
+    torch = _torch()
+    hd, tokens = kcache.shape[-1], q.shape[0]
+    _on_device(q, k, v, kcache, vcache, page_table, row_start, context, cos, sin, q_out)
+    if q.dim() != 2 or k.shape != v.shape or k.dim() != 2 or k.shape[0] != tokens or k.shape[1] != kcache.shape[2] * hd or q.shape[1] % hd:
+        raise ValueError("q [tokens, n_heads_q * head_dim], k and v [tokens, n_heads_kv * head_dim]")
+    if q.dtype != torch.float32 or k.dtype != torch.float32 or v.dtype != torch.float32 or k.stride() != v.stride() or q.stride(1) != 1 or k.stride(1) != 1:
+        raise ValueError("q, k and v: fp32 rows; those of k and v at the same distance")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != hd:
+        raise ValueError("cos and sin: [positions, head_dim]")
+    hq = q.shape[1] // hd
+    c, b, _ = _paged(kcache, vcache, hq, page_table, row_start, context, tokens, max_new, 0)
+    if q_out is None:
+        q_out = torch.empty((tokens, hq, hd), dtype=kcache.dtype, device=q.device)
+    elif q_out.dtype != kcache.dtype or q_out.shape != (tokens, hq, hd) or q_out.stride(2) != 1 or q_out.stride(1) != hd:
+        raise ValueError("q_out: [tokens, n_heads_q, head_dim] in the caches' type")
+    qg, kg, eps = qk_norm if qk_norm is not None else (None, None, 0.0)
+    _on_device(qg, kg)
+    check(lib().nntr_cuda_paged_append_dev(
+        c, b, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), _typed(qg, "q_gamma", torch.float32, hd),
+        _typed(kg, "k_gamma", torch.float32, hd), eps, _typed(cos, "cos", torch.float32), _typed(sin, "sin", torch.float32), cos.shape[0],
+        q_out.data_ptr(), q_out.stride(0), _flags(pdl), _stream()))
+    return q_out
+
+
+def paged_attention(q, kcache, vcache, page_table, row_start, context, max_new: int, max_rows: int = 0, window: int | None = None,
+                    first_tokens: int = 0, sink=None, out=None, pdl: bool = False):
+    """Attention of the new tokens of a batch of sequences (one each, or chunks) over a cache in pages that holds their rows already.
+    q [tokens, n_heads_q, head_dim] in the caches' type; kcache, vcache [n_pages, page_size, n_heads_kv, head_dim]. Sequence b has
+    the rows row_start[b] .. row_start[b + 1] of q, which are the last of its context[b] rows; row r lies in page
+    page_table[b, r // page_size] (int32 device tensors). ``max_new``: rows of the longest sequence at most; ``max_rows``: about the longest
+    context, 0 if not known (it chooses how the work is split). A query at position p sees rows j <= p with j > p - window or
+    j < first_tokens; ``sink``: fp32 logits [n_heads_q]. ``out``: [tokens, n_heads_q, head_dim] in the caches' type (made if None) or
+    fp32, the form the projections take; rows behind the last sequence are left as they are."""
+    torch = _torch()
+    _on_device(q, kcache, vcache, page_table, row_start, context, sink, out)
+    if q.dim() != 3 or q.shape[2] != kcache.shape[-1] or q.dtype != kcache.dtype or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        raise ValueError("q: [tokens, n_heads_q, head_dim] in the caches' type")
+    tokens, hq, hd = q.shape
+    c, b, dtype = _paged(kcache, vcache, hq, page_table, row_start, context, tokens, max_new, max_rows)
+    if out is None:
+        out = torch.empty((tokens, hq, hd), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != hd or out.dtype not in (q.dtype, torch.float32):
+        raise ValueError("out: [tokens, n_heads_q, head_dim] in the caches' type or fp32")
+    check(lib().nntr_cuda_paged_attention_dev(
+        c, b, q.data_ptr(), q.stride(0), 0xFFFFFFFF if window is None else window, first_tokens, _typed(sink, "sink", torch.float32, hq),
+        out.data_ptr(), capi.F32 if out.dtype == torch.float32 else dtype, out.stride(0), _flags(pdl), _stream()))
+    return out
+
+
+def copy_pages(caches, src, dst, pdl: bool = False) -> None:
+    """Pages src[i] -> dst[i] in every array of ``caches`` ([..., n_pages, page_size, n_heads_kv, head_dim], contiguous: the key and
+    value caches of all layers), in one launch. src and dst: int32 device tensors; no page twice in dst, or in both."""
+    torch = _torch()
+    _on_device(caches, src, dst)
+    if caches.dim() < 4 or not caches.is_contiguous():
+        raise ValueError("caches: a contiguous [..., n_pages, page_size, n_heads_kv, head_dim]")
+    n = src.numel()
+    page = caches.stride(-4) * caches.element_size()
+    pages = caches.shape[-4]
+    check(lib().nntr_cuda_copy_pages_dev(caches.data_ptr(), caches.numel() // (caches.stride(-4) * pages) if n else 0, page * pages, page, pages,
+                                         _typed(src, "src", torch.int32), _typed(dst, "dst", torch.int32, n), n, _flags(pdl), _stream()))
+
+
+def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, params=None, out=(None, None, None),
+           pdl: bool = False):
+    """A token per row of ``logits`` (fp32, over the last dimension) from the random numbers ``u`` in [0, 1), one per row: temperature,
+    top_k (0: off), top_p (1: off) and min_p (0: off), applied in that order (nntr_cuda_sample_dev). ``params``: fp32 [rows, 4] of the four for
+    each row instead. Returns (uint32 indices as an int32 tensor, the same as float32, the tokens' probabilities among the kept)."""
+    torch = _torch()
+    _on_device(logits, u, params)
+    n = logits.shape[-1]
+    if logits.dtype != torch.float32 or logits.stride(-1) != 1 or (logits.dim() > 2 and not logits.is_contiguous()):
+        raise ValueError("logits: fp32 [rows, n]")
+    rows = logits.numel() // n if n else 0
+    ld = logits.stride(0) if logits.dim() == 2 else n
+    new = lambda t, dt: torch.empty(rows, dtype=dt, device=logits.device) if t is None else t  # noqa: E731
+    idx, idx_f, prob = new(out[0], torch.int32), new(out[1], torch.float32), new(out[2], torch.float32)
+    _on_device(idx, idx_f, prob)
+    check(lib().nntr_cuda_sample_dev(
+        logits.data_ptr(), rows, n, ld, _typed(u, "u", torch.float32, rows), temperature, top_k, top_p, min_p,
+        _typed(params, "params", torch.float32, 4 * rows), _typed(idx, "out", torch.int32, rows), _typed(idx_f, "out", torch.float32, rows),
+        _typed(prob, "out", torch.float32, rows), _flags(pdl), _stream()))
+    return idx, idx_f, prob
+
+
+class PagedCache:
+    """The key and value caches of all layers in pages, and which sequence holds which page: ``kv`` [layers, 2, n_pages, page_size,
+    n_heads_kv, head_dim]. A sequence that forks shares its full pages with the new one; the page that it is in the middle of is copied, so a
+    shared page is never written. Sequences are small integers. The counts live on the host; only ``fork`` and ``compact`` launch copies,
+    on the current stream."""
+
+    def __init__(self, n_layers: int, n_pages: int, page_size: int, n_heads_kv: int, head_dim: int, dtype=None, device="cuda"):
+        torch = _torch()
+        self.n_pages, self.page_size, self.device = n_pages, page_size, device
+        self.kv = torch.zeros((n_layers, 2, n_pages, page_size, n_heads_kv, head_dim), dtype=dtype or torch.float16, device=device)
+        self._refs = [0] * n_pages
+        self._free = list(range(n_pages - 1, -1, -1))  # handed out from the end
+        self._seqs: dict[int, list] = {}  # sequence -> [rows, pages]
+        self._next = 0
+
+    def keys(self, layer: int):
+        return self.kv[layer, 0]
+
+    def values(self, layer: int):
+        return self.kv[layer, 1]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def rows(self, seq: int) -> int:
+        return self._seqs[seq][0]
+
+    def pages(self, seq: int) -> list:
+        return list(self._seqs[seq][1])
+
+    def _take(self, n: int) -> list:
+        if n > len(self._free):
+            raise MemoryError(f"{n} pages needed, {len(self._free)} of {self.n_pages} free")
+        pages = [self._free.pop() for _ in range(n)]
+        for p in pages:
+            self._refs[p] = 1
+        return pages
+
+    def _copy(self, src: list, dst: list) -> None:
+        torch = _torch()
+        if src:
+            both = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
+            copy_pages(self.kv, both[0], both[1])
+
+    def new(self) -> int:
+        """A sequence without rows."""
+        seq, self._next = self._next, self._next + 1
+        self._seqs[seq] = [0, []]
+        return seq
+
+    def reserve(self, seqs, new) -> None:
+        """Room for new[i] more rows of seqs[i]; MemoryError, with nothing changed, if the pool has too few pages."""
+        seqs, new = list(seqs), list(new)
+        if len(set(seqs)) != len(seqs) or len(seqs) != len(new) or any(n < 0 for n in new):
+            raise ValueError("reserve: each sequence once, with a number of rows")
+        need = [max(0, -(-(self._seqs[s][0] + n) // self.page_size) - len(self._seqs[s][1])) for s, n in zip(seqs, new)]
+        pages = self._take(sum(need))
+        for s, n, k in zip(seqs, new, need):
+            self._seqs[s][0] += n
+            self._seqs[s][1] += pages[:k]
+            del pages[:k]
+
+    def batch(self, seqs, new) -> dict:
+        """The arrays of a call in which the last new[i] rows of seqs[i] are the new tokens: keyword arguments of ``paged_append`` (without
+        max_rows) and ``paged_attention``."""
+        torch = _torch()
+        seqs, new = list(seqs), list(new)
+        if not seqs or len(seqs) != len(new) or any(not 0 <= n <= self._seqs[s][0] for s, n in zip(seqs, new)):
+            raise ValueError("batch: no sequence has more new rows than rows")
+        wide = max(1, max(len(self._seqs[s][1]) for s in seqs))
+        words, at = [0], 0
+        for n in new:
+            at += n
+            words.append(at)
+        words += [self._seqs[s][0] for s in seqs]
+        for s in seqs:
+            pages = self._seqs[s][1]
+            words += pages + [-1] * (wide - len(pages))
+        t = torch.tensor(words, dtype=torch.int32).to(self.device)  # one transfer
+        b = len(seqs)
+        return dict(row_start=t[:b + 1], context=t[b + 1:2 * b + 1], page_table=t[2 * b + 1:].view(b, wide), max_new=max(new),
+                    max_rows=max(self._seqs[s][0] for s in seqs))
+
+    def fork(self, seq: int, n: int = 1) -> list:
+        """n new sequences with the rows of ``seq``."""
+        rows, pages = self._seqs[seq]
+        full = rows // self.page_size
+        part = pages[full:]  # the page that the rows end in, if they end inside one
+        fresh = self._take(n * len(part))
+        out = []
+        for i in range(n):
+            s = self.new()
+            own = fresh[i * len(part):(i + 1) * len(part)]
+            self._seqs[s] = [rows, pages[:full] + own]
+            for p in pages[:full]:
+                self._refs[p] += 1
+            out.append(s)
+        self._copy(part * n, fresh)
+        return out
+
+    def free(self, seq: int) -> None:
+        """Gives the sequence up; pages that no other one shares return to the pool."""
+        for p in self._seqs.pop(seq)[1]:
+            self._refs[p] -= 1
+            if not self._refs[p]:
+                self._free.append(p)
+
+    def compact(self) -> int:
+        """Moves pages so that the used ones are the lowest of the pool; returns how many moved. Arrays of ``batch`` made before are stale."""
+        used = sum(r > 0 for r in self._refs)
+        holes = [p for p in range(used) if not self._refs[p]]
+        src = [p for p in range(used, self.n_pages) if self._refs[p]]
+        to = dict(zip(src, holes))
+        self._copy(src, holes)
+        for held in self._seqs.values():
+            held[1] = [to.get(p, p) for p in held[1]]
+        for a, b in to.items():
+            self._refs[b], self._refs[a] = self._refs[a], 0
+        self._free = list(range(self.n_pages - 1, used - 1, -1))
+        return len(src)
+
+
 # --------------------------------------------------------- .bin weight files
 _BIN_DTYPE = {"f32": capi.F32, "f16": capi.F16, "q4_0": capi.Q4_0, "q4_K": capi.Q4_K, "q6_K": capi.Q6_K}
 

@@ -57,6 +57,10 @@ SIGNATURES = {
                                           _vp, _sz, _u, _vp]),
     "nntr_cuda_attention_rows_dev": (_i, [_vp, _u, _u, _u, _vp, _vp, _vp, _sz, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp, _sz,
                                           _u, _vp]),
+    "nntr_cuda_paged_append_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, C.c_float, _vp, _vp, _u, _vp, _i64, _u, _vp]),
+    "nntr_cuda_paged_attention_dev": (_i, [_vp, _vp, _vp, _i64, _u, _u, _vp, _vp, _i, _i64, _u, _vp]),
+    "nntr_cuda_copy_pages_dev": (_i, [_vp, _u, _i64, _i64, _u, _vp, _vp, _u, _u, _vp]),
+    "nntr_cuda_sample_dev": (_i, [_vp, _i64, _i64, _i64, _vp, C.c_double, _u, C.c_double, C.c_double, _vp, _vp, _vp, _vp, _u, _vp]),
     "nntr_cuda_bin_layout": (_i, [_vp, _sz, _vp, _vp, _vp]),
     "nntr_cuda_bin_load": (_i, [C.c_char_p, _vp, _sz, _i, _i, _vp, _vp]),
     "nntr_cuda_quantize_q8_K_dev": (_i, [_vp, _i64, _vp, _i64, _i64, _i, _vp]),
@@ -126,12 +130,24 @@ class AttnDesc(C.Structure):
                 ("sink", C.c_void_p)]
 
 
+class PagedCache(C.Structure):
+    """nntr_paged_cache of include/nntr_cuda.h."""
+    _fields_ = [("n_heads_q", C.c_uint), ("n_heads_kv", C.c_uint), ("head_dim", C.c_uint), ("dtype", C.c_int), ("page_size", C.c_uint),
+                ("n_pages", C.c_uint), ("page_stride", C.c_int64), ("kcache", C.c_void_p), ("vcache", C.c_void_p)]
+
+
+class PagedBatch(C.Structure):
+    """nntr_paged_batch of include/nntr_cuda.h."""
+    _fields_ = [("batch", C.c_uint), ("tokens", C.c_uint), ("max_new", C.c_uint), ("max_rows", C.c_uint), ("ld_table", C.c_uint),
+                ("row_start", C.c_void_p), ("context", C.c_void_p), ("page_table", C.c_void_p)]
+
+
 class BinTensor(C.Structure):
     """nntr_bin_tensor of include/nntr_cuda.h."""
     _fields_ = [("dtype", C.c_int), ("N", C.c_uint), ("K", C.c_uint)]
 
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 30
 
 
 class MoeEp(C.Structure):

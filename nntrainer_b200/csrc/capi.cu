@@ -556,6 +556,11 @@ int nntr_cuda_device_status(void) {
     return rc;
   if (v)
     return set_error(v, "an embedding lookup met a token index beyond its table");
+  if ((rc = read_paged_cache_status(&v, false)) || (!v && (rc = read_paged_attn_status(&v, false))))
+    return rc;
+  if (v)
+    return v == NNTR_CUDA_ERR_TIMEOUT ? set_error(v, "a device kernel gave up on a bounded wait (status %d)", v)
+                                      : set_error(v, "the rows, contexts or pages of a paged call contradict its bounds");
   return NNTR_CUDA_OK;
 }
 
@@ -584,7 +589,9 @@ int nntr_cuda_clear_device_status(void) {
   NNTR_CHECK_CUDA(cudaDeviceSynchronize());
   int v = 0;
   int rc = read_embed_status(&v, true);
-  return rc ? rc : clear_device_status_words();
+  if (rc || (rc = read_paged_cache_status(&v, true)) || (rc = read_paged_attn_status(&v, true)))
+    return rc;
+  return clear_device_status_words();
 }
 
 int nntr_cuda_set_exchange_poll_limit(unsigned polls) { return set_exchange_poll_limit(polls); }
@@ -669,6 +676,30 @@ int nntr_cuda_attention_rows_dev(const nntr_attn_desc *a, unsigned pos, unsigned
   return launch_attention_rows(a, pos, tokens, max_rows, q, k, v, ld, q_gamma, k_gamma, eps, static_cast<uint16_t *>(kcache),
                                static_cast<uint16_t *>(vcache), cos_tab, sin_tab, out, ld_out, flags,
                                static_cast<cudaStream_t>(stream));
+}
+
+int nntr_cuda_paged_append_dev(const nntr_paged_cache *c, const nntr_paged_batch *b, const float *q, const float *k, const float *v,
+                               int64_t ld_q, int64_t ld_kv, const float *q_gamma, const float *k_gamma, float eps,
+                               const float *cos_tab, const float *sin_tab, unsigned table_rows, void *q_out, int64_t ld_out,
+                               unsigned flags, void *stream) {
+  return launch_paged_append(c, b, q, k, v, ld_q, ld_kv, q_gamma, k_gamma, eps, cos_tab, sin_tab, table_rows, q_out, ld_out, flags,
+                             static_cast<cudaStream_t>(stream));
+}
+int nntr_cuda_paged_attention_dev(const nntr_paged_cache *c, const nntr_paged_batch *b, const void *q, int64_t ld_q,
+                                  unsigned window, unsigned first_tokens, const float *sink, void *out, int out_dtype,
+                                  int64_t ld_out, unsigned flags, void *stream) {
+  return launch_paged_attention(c, b, q, ld_q, window, first_tokens, sink, out, out_dtype, ld_out, flags,
+                                static_cast<cudaStream_t>(stream));
+}
+int nntr_cuda_copy_pages_dev(void *base, unsigned arrays, int64_t array_bytes, int64_t page_bytes, unsigned n_pages, const int *src,
+                             const int *dst, unsigned n, unsigned flags, void *stream) {
+  return launch_copy_pages(base, arrays, array_bytes, page_bytes, n_pages, src, dst, n, flags, static_cast<cudaStream_t>(stream));
+}
+int nntr_cuda_sample_dev(const float *logits, int64_t rows, int64_t n, int64_t ld, const float *u, double temperature, unsigned top_k,
+                         double top_p, double min_p, const float *row_params, unsigned *idx_out, float *idx_out_f, float *prob_out,
+                         unsigned flags, void *stream) {
+  return launch_sample(logits, rows, n, ld, u, temperature, top_k, top_p, min_p, row_params, idx_out, idx_out_f, prob_out, flags,
+                       static_cast<cudaStream_t>(stream));
 }
 
 int nntr_cuda_bin_layout(const nntr_bin_tensor *t, size_t n, size_t *data_offset, size_t *bytes, size_t *total) {

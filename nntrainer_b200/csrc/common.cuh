@@ -397,6 +397,18 @@ int launch_argmax(const float *x, long long rows, long long n, long long ld, uns
 int launch_embedding(int qtype, const void *table, const float *ids, float *y, unsigned n_ids, unsigned in_dim,
                      unsigned out_dim, unsigned flags, cudaStream_t st);
 int read_embed_status(int *out, bool clear);
+int read_paged_cache_status(int *out, bool clear);
+int read_paged_attn_status(int *out, bool clear);
+int launch_paged_append(const nntr_paged_cache *c, const nntr_paged_batch *b, const float *q, const float *k, const float *v,
+                        int64_t ld_q, int64_t ld_kv, const float *q_gamma, const float *k_gamma, float eps, const float *cos_tab,
+                        const float *sin_tab, unsigned table_rows, void *q_out, int64_t ld_out, unsigned flags, cudaStream_t st);
+int launch_paged_attention(const nntr_paged_cache *c, const nntr_paged_batch *b, const void *q, int64_t ld_q, unsigned window,
+                           unsigned first_tokens, const float *sink, void *out, int out_dtype, int64_t ld_out, unsigned flags,
+                           cudaStream_t st);
+int launch_copy_pages(void *base, unsigned arrays, int64_t array_bytes, int64_t page_bytes, unsigned n_pages, const int *src,
+                      const int *dst, unsigned n, unsigned flags, cudaStream_t st);
+int launch_sample(const float *logits, int64_t rows, int64_t n, int64_t ld, const float *u, double temperature, unsigned top_k, double top_p,
+                  double min_p, const float *row_params, unsigned *idx, float *idx_f, float *prob, unsigned flags, cudaStream_t st);
 /* single-token attention (attention.cu) */
 int launch_rope_cache_append(const nntr_attn_desc *a, unsigned pos, const unsigned *pos_dev, float *q, const float *k,
                              const float *v, const float *q_gamma, const float *k_gamma, float eps, uint16_t *kcache,

@@ -1,0 +1,407 @@
+// SPDX-License-Identifier: Apache-2.0
+/**
+ * @file  paged_attention.cu
+ * @brief Attention of the new tokens of a batch of sequences over a key/value cache in pages: few tokens of a sequence (one, or a
+ *        draft's) here; launch_paged_attention() is the entry for all.
+ *
+ *   s_j = q . k_j / sqrt(head_dim) for the rows j the query at position p sees: j <= p and (j > p - window or j < first_tokens)
+ *   out = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m)), m = max_j s_j; zeros where nothing is seen
+ *
+ * Scores, maxima, sums and results are fp32. The probabilities are rounded to the cache's 16-bit type, the operand type of the
+ * tensor cores (2^-11 or 2^-8 of each, which the sum over the rows averages out); fp16 ones are kept 2^10 times as large, so
+ * that the small ones of a long context stay out of its subnormal numbers.
+ */
+#include "cluster.cuh"
+#include "paged.cuh"
+#include "pipeline.cuh"
+
+#include <algorithm>
+
+namespace nntr {
+
+__device__ int g_paged_attn_status = 0;
+
+int read_paged_attn_status(int *out, bool clear) {
+  int v = 0;
+  NNTR_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_paged_attn_status, sizeof(int)));
+  if (v && clear) {
+    const int zero = 0;
+    NNTR_CHECK_CUDA(cudaMemcpyToSymbol(g_paged_attn_status, &zero, sizeof(int)));
+  }
+  *out = v;
+  return NNTR_CUDA_OK;
+}
+
+struct AttendArgs {
+  const void *q, *k, *v;
+  void *out;
+  const float *sink;
+  long long ld_q, ld_out;
+  int window, first; // window: INT_MAX / 2 where there is none
+  int out_f32;
+  float scale_log2; // log2(e) / sqrt(head_dim)
+};
+
+/* ------------------------------------------------------ a few query rows */
+
+/* Rows of a tile are (token, query head of the kv head's group), 16 of them: one M of the warp MMA. Every warp takes blocks of 16
+ * cache rows in turn through a ring of its own, so that nothing but the end is shared: cp.async for block i + stages, scores of
+ * block i, probabilities straight from the accumulators to the operand of the second product. The warps of a CTA join through
+ * shared memory, the CTAs of a cluster, which share the cache rows of one (sequence, kv head, tile), through each other's.
+ * Bandwidth bounds it: 2 * 2 * head_dim bytes per cache row and kv head. */
+constexpr int PD_WARPS = 4;
+constexpr int PD_KEYS = 16; // of a block: no more than the smallest page
+template <int HD> struct PdCfg {
+  static constexpr int STAGES = HD == 128 ? 3 : 6;
+  static constexpr int KV_BYTES = PD_KEYS * HD * 2;
+  static constexpr int RING = STAGES * 2 * KV_BYTES;              // of a warp
+  static constexpr int PART = (16 * HD + 32) * 4;                 // O, m, l of a warp or a CTA
+  static constexpr int SMEM = PD_WARPS * (RING > PART ? RING : PART) + PART;
+};
+
+template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+/* 16 bytes to shared memory, zeros where `bytes` is 0 (nothing is read then) */
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+/* Blocks of KEYS cache rows that hold what a tile of queries at positions lo .. hi sees: those of the first tokens, then the window's.
+ * A row in none of the queries' sight counts as not there: it may hold anything. */
+struct Sight {
+  int lo, hi, window, first, from, head_blocks, first_block, blocks;
+  __device__ __forceinline__ Sight(int lo_, int hi_, int window_, int first_, int keys) : lo(lo_), hi(hi_), window(window_) {
+    from = max(0, lo - window + 1);
+    first = min(first_, from);
+    head_blocks = (first + keys - 1) / keys;
+    first_block = from / keys;
+    if (first_block <= head_blocks)
+      head_blocks = first_block = 0;
+    blocks = hi < 0 ? 0 : head_blocks + hi / keys - first_block + 1;
+  }
+  __device__ __forceinline__ int block(int i) const { return i < head_blocks ? i : i - head_blocks + first_block; }
+  __device__ __forceinline__ bool row_read(int j) const { return j <= hi && (j >= from || j < first); } // by one query at least
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(AttendArgs a, PagedGeom g, PagedBatch s) {
+  using Cfg = PdCfg<HD>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int parts = cluster_size(), part = cluster_rank();
+  const int tile = blockIdx.x / parts, h = blockIdx.y, seq = blockIdx.z;
+  pdl_launch_dependents();
+  pdl_wait();
+  const SeqRows r = seq_rows(s, seq);
+  if (r.bad && threadIdx.x == 0)
+    atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
+  const int G = g.hq / g.hkv, rows = min(16, r.n * G - tile * 16);
+  if (rows <= 0)
+    return; // every CTA of the cluster alike
+  const int tok0 = tile * 16 / G, tok1 = (tile * 16 + rows - 1) / G;
+  const Sight sight(r.pos + tok0, r.pos + tok1, a.window, a.first, PD_KEYS);
+
+  // this lane's two rows: lane / 4 and 8 more
+  const int gr = lane >> 2, gc = lane & 3;
+  int row_pos[2];
+  uint32_t qf[HD / 16][4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int row = gr + 8 * k, flat = tile * 16 + row, tok = flat / G;
+    row_pos[k] = row < rows ? r.pos + tok : -1;
+    const T *qr = static_cast<const T *>(a.q) + (r.first + min(tok, tok1)) * a.ld_q + (size_t)(h * G + flat % G) * g.hd;
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int col = 16 * c + 8 * u + 2 * gc;
+        qf[c][k + 2 * u] = row < rows && col < g.hd ? *reinterpret_cast<const uint32_t *>(qr + col) : 0u;
+      }
+  }
+
+  const uint32_t ring = smem_u32(smem) + warp * Cfg::RING;
+  const int n_mine = sight.blocks > part * PD_WARPS + warp ? (sight.blocks - part * PD_WARPS - warp + parts * PD_WARPS - 1) / (parts * PD_WARPS) : 0;
+  auto my_block = [&](int i) { return sight.block((i * parts + part) * PD_WARPS + warp); };
+  // a lane keeps the address of one of the next 32 blocks, so that the way over the page table is taken once for all of them
+  long long at = 0;
+  auto fetch = [&](int i) {
+    if (i < n_mine) {
+      if (i % 32 == 0)
+        at = i + lane < n_mine ? g.row_offset(s, seq, my_block(i + lane) * PD_KEYS, h) : 0;
+      const long long off = __shfl_sync(FULL, at, i % 32);
+      const int j0 = my_block(i) * PD_KEYS;
+      if (off < 0 && lane == 0)
+        atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
+      constexpr int CHUNKS = HD / 8; // of a row
+      const uint32_t dst = ring + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES;
+#pragma unroll
+      for (int u = 0; u < PD_KEYS * CHUNKS / 32; ++u) {
+        const int c = lane % CHUNKS, row = lane / CHUNKS + u * (32 / CHUNKS);
+        const bool there = off >= 0 && sight.row_read(j0 + row) && 8 * c < g.hd;
+        const long long e = there ? off + (long long)row * g.hkv * g.hd + 8 * c : 0;
+        const uint32_t to = dst + row * (HD * 2) + ((c ^ (row & 7)) << 4); // rows' pieces spread over the banks for ldmatrix
+        cp16(to, static_cast<const T *>(a.k) + e, there ? 16 : 0);
+        cp16(to + Cfg::KV_BYTES, static_cast<const T *>(a.v) + e, there ? 16 : 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < HD / 8; ++c)
+    o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+  constexpr float LIFT = 10.f; // log2 of the factor of the probabilities
+  for (int i = 0; i < Cfg::STAGES - 1; ++i)
+    fetch(i);
+  for (int i = 0; i < n_mine; ++i) {
+    fetch(i + Cfg::STAGES - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::STAGES - 1) : "memory");
+    __syncwarp();
+    const uint32_t kt = ring + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES, vt = kt + Cfg::KV_BYTES;
+    const int j0 = my_block(i) * PD_KEYS;
+    float sc[2][4] = {};
+    { // four 8 x 8 matrices: keys 0-7 and 8-15, each with the lower and the upper 8 of 16 dimensions
+      const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+      for (int c = 0; c < HD / 16; ++c) {
+        uint32_t b[4];
+        ldsm4(b, kt + row * (HD * 2) + (((2 * c + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+        mma16816<T>(sc[0], qf[c], b[0], b[1]);
+        mma16816<T>(sc[1], qf[c], b[2], b[3]);
+      }
+    }
+    const bool whole = j0 + PD_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PD_KEYS <= a.first);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = j0 + 8 * t + 2 * gc + (e & 1), p = row_pos[e >> 1];
+        sc[t][e] = whole || (j <= p && (j > p - a.window || j < a.first)) ? sc[t][e] * a.scale_log2 : -INFINITY;
+      }
+    uint32_t pf[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) { // the lane's two rows
+      float mx = fmaxf(fmaxf(sc[0][2 * k], sc[0][2 * k + 1]), fmaxf(sc[1][2 * k], sc[1][2 * k + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
+      mx = fmaxf(mx, m[k]);
+      const float base = mx == -INFINITY ? 0.f : mx - LIFT; // nothing seen yet: all weights are exp2(-inf)
+      const float turn = ex2(m[k] - mx); // m = mx = -inf: NaN, replaced below
+      const float keep = m[k] == mx ? 1.f : turn;
+      m[k] = mx;
+      const float p0 = ex2(sc[0][2 * k] - base), p1 = ex2(sc[0][2 * k + 1] - base), p2 = ex2(sc[1][2 * k] - base),
+                  p3 = ex2(sc[1][2 * k + 1] - base);
+      l[k] = l[k] * keep + ((p0 + p1) + (p2 + p3));
+      pf[k] = pack2<T>(p0, p1);
+      pf[k + 2] = pack2<T>(p2, p3);
+      if (__any_sync(FULL, keep != 1.f))
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          o[c][2 * k] *= keep;
+          o[c][2 * k + 1] *= keep;
+        }
+    }
+    { // keys 0-7 and 8-15 of eight dimensions, then of the next eight
+      const int row = lane & 15;
+#pragma unroll
+      for (int c = 0; c < HD / 16; ++c) {
+        uint32_t b[4];
+        ldsm4t(b, vt + row * (HD * 2) + (((2 * c + (lane >> 4)) ^ (row & 7)) << 4));
+        mma16816<T>(o[2 * c], pf, b[0], b[1]);
+        mma16816<T>(o[2 * c + 1], pf, b[2], b[3]);
+      }
+    }
+    __syncwarp(); // the slot is read: the copies of the next round may fill it
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    l[k] += __shfl_xor_sync(FULL, l[k], 1);
+    l[k] += __shfl_xor_sync(FULL, l[k], 2);
+  }
+
+  /* ---- the warps' parts, then the CTAs': each a row's O, m and l; the ring is free */
+  __syncthreads();
+  float *mine = reinterpret_cast<float *>(smem) + warp * (Cfg::PART / 4);
+#pragma unroll
+  for (int c = 0; c < HD / 8; ++c)
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      *reinterpret_cast<float2 *>(mine + (gr + 8 * k) * HD + 8 * c + 2 * gc) = make_float2(o[c][2 * k], o[c][2 * k + 1]);
+  if (gc == 0)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      mine[16 * HD + gr + 8 * k] = m[k];
+      mine[16 * HD + 16 + gr + 8 * k] = l[k];
+    }
+  __syncthreads();
+  // sum of n parts: part i of a value is at(i, element); returns the row's denominator by *total
+  auto joined = [&](int n, auto part_of, int row, int col, float *mx, float *total) {
+    float big = -INFINITY;
+    for (int i = 0; i < n; ++i)
+      big = fmaxf(big, part_of(i, 16 * HD + row, 1).x);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float lsum = 0.f;
+    for (int i = 0; i < n; ++i) {
+      const float mi = part_of(i, 16 * HD + row, 1).x, w = mi == -INFINITY ? 0.f : ex2(mi - big);
+      const float4 v = part_of(i, row * HD + col, 4);
+      lsum += w * part_of(i, 16 * HD + 16 + row, 1).x;
+      sum = make_float4(sum.x + w * v.x, sum.y + w * v.y, sum.z + w * v.z, sum.w + w * v.w);
+    }
+    *mx = big;
+    *total = lsum;
+    return sum;
+  };
+  constexpr int OWN = PD_WARPS * (Cfg::RING > Cfg::PART ? Cfg::RING : Cfg::PART); // bytes in front of the CTA's part
+  float *cta = reinterpret_cast<float *>(smem + OWN);
+  auto of_warp = [&](int i, int e, int n) {
+    const float *p = reinterpret_cast<const float *>(smem) + i * (Cfg::PART / 4) + e;
+    return n == 4 ? *reinterpret_cast<const float4 *>(p) : make_float4(*p, 0.f, 0.f, 0.f);
+  };
+  const uint32_t cta_addr = smem_u32(cta);
+  auto of_cta = [&](int i, int e, int n) {
+    if (n == 4)
+      return ld_cluster4(cta_addr + 4u * e, i);
+    uint32_t remote;
+    float x;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(cta_addr + 4u * e), "r"(i));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote) : "memory");
+    return make_float4(x, 0.f, 0.f, 0.f);
+  };
+  auto store = [&](int row, int col, const float4 &sum, float mx, float total) {
+    const int flat = tile * 16 + row, head = h * G + flat % G;
+    if (a.sink && mx > -INFINITY)
+      total += ex2(a.sink[head] * 1.4426950408889634f - (mx - LIFT));
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float4 f = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+    const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd + col;
+    if (a.out_f32)
+      *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + e) = f;
+    else
+      *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + e) = make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
+  };
+  for (int i = threadIdx.x; i < 16 * HD / 4; i += PD_WARPS * 32) {
+    const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
+    if (row >= rows || col >= g.hd)
+      continue;
+    float mx, total;
+    const float4 sum = joined(PD_WARPS, of_warp, row, col, &mx, &total);
+    if (parts == 1) {
+      store(row, col, sum, mx, total);
+      continue;
+    }
+    *reinterpret_cast<float4 *>(cta + row * HD + col) = sum;
+    if (col == 0) {
+      cta[16 * HD + row] = mx;
+      cta[16 * HD + 16 + row] = total;
+    }
+  }
+  if (parts == 1)
+    return;
+  cluster_sync();
+  for (int i = part * PD_WARPS * 32 + threadIdx.x; i < 16 * HD / 4; i += parts * PD_WARPS * 32) {
+    const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
+    if (row >= rows || col >= g.hd)
+      continue;
+    float mx, total;
+    const float4 sum = joined(parts, of_cta, row, col, &mx, &total);
+    store(row, col, sum, mx, total);
+  }
+  cluster_sync(); // nobody leaves while its part is read
+}
+
+/* ------------------------------------------------------------------ launch */
+
+template <typename T, int HD>
+static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch &s, int parts, int tiles, unsigned flags, cudaStream_t st) {
+  auto kernel = paged_attention_few_kernel<T, HD>;
+  constexpr int smem = PdCfg<HD>::SMEM;
+  NNTR_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = {};
+  cfg.attrs = attr;
+  cfg.numAttrs = 0;
+  if (parts > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = parts;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (flags & NNTR_CUDA_GEMV_PDL) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.gridDim = dim3((unsigned)(tiles * parts), (unsigned)g.hkv, (unsigned)s.batch);
+  cfg.blockDim = dim3(PD_WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, g, s);
+  count_launch();
+  return check_cuda(e, "paged_attention launch");
+}
+
+int launch_paged_attention(const nntr_paged_cache *c, const nntr_paged_batch *b, const void *q, int64_t ld_q, unsigned window,
+                           unsigned first_tokens, const float *sink, void *out, int out_dtype, int64_t ld_out, unsigned flags,
+                           cudaStream_t st) {
+  PagedGeom g;
+  PagedBatch s;
+  int rc = check_paged("paged_attention", c, b, &g, &s);
+  if (rc)
+    return rc;
+  if (s.batch == 0 || s.tokens == 0 || s.max_new == 0)
+    return NNTR_CUDA_OK;
+  if (!q || !out)
+    return set_error(NNTR_CUDA_ERR_INVALID, "paged_attention: null pointer");
+  if (out_dtype != c->dtype && out_dtype != NNTR_F32)
+    return set_error(NNTR_CUDA_ERR_UNSUPPORTED, "paged_attention: results of the cache's type or fp32 (dtype %d)", out_dtype);
+  const int64_t width = (int64_t)g.hq * g.hd;
+  if (ld_q < width || ld_q % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || ld_out < width || ld_out % 8 || (reinterpret_cast<uintptr_t>(out) & 15))
+    return set_error(NNTR_CUDA_ERR_INVALID, "paged_attention: rows of %lld elements, %lld and %lld apart; need 16-byte aligned rows that do not overlap",
+                     (long long)width, (long long)ld_q, (long long)ld_out);
+  if (window == 0)
+    return set_error(NNTR_CUDA_ERR_INVALID, "paged_attention: a window of no rows");
+  constexpr int NONE = 0x3fffffff;
+  AttendArgs a = {q, c->kcache, c->vcache, out, sink, ld_q, ld_out, (int)std::min(window, (unsigned)NONE),
+                  (int)std::min(first_tokens, (unsigned)NONE), out_dtype == NNTR_F32, 1.4426950408889634f / sqrtf((float)g.hd)};
+  const int G = g.hq / g.hkv, tiles = (int)(((long long)s.max_new * G + 15) / 16);
+  const long long items = (long long)tiles * g.hkv * s.batch;
+  long long seen = std::min<long long>((long long)a.window + a.first + s.max_new, b->max_rows ? b->max_rows : NONE);
+  const long long blocks = (seen + PD_KEYS - 1) / PD_KEYS;
+  int parts = 1;
+  while (parts < 8 && items * parts < 2 * sm_count() && blocks >= 2ll * 2 * parts * PD_WARPS)
+    parts *= 2;
+  if (c->dtype == NNTR_F16)
+    return g.hd <= 64 ? launch_few<__half, 64>(a, g, s, parts, tiles, flags, st) : launch_few<__half, 128>(a, g, s, parts, tiles, flags, st);
+  return g.hd <= 64 ? launch_few<__nv_bfloat16, 64>(a, g, s, parts, tiles, flags, st)
+                    : launch_few<__nv_bfloat16, 128>(a, g, s, parts, tiles, flags, st);
+}
+
+} // namespace nntr

@@ -556,7 +556,8 @@ int nntr_cuda_device_status(void) {
     return rc;
   if (v)
     return set_error(v, "an embedding lookup met a token index beyond its table");
-  if ((rc = read_paged_cache_status(&v, false)) || (!v && (rc = read_paged_attn_status(&v, false))))
+  if ((rc = read_paged_cache_status(&v, false)) || (!v && (rc = read_paged_attn_status(&v, false))) ||
+      (!v && (rc = read_paged_chunk_status(&v, false))))
     return rc;
   if (v)
     return v == NNTR_CUDA_ERR_TIMEOUT ? set_error(v, "a device kernel gave up on a bounded wait (status %d)", v)
@@ -589,7 +590,7 @@ int nntr_cuda_clear_device_status(void) {
   NNTR_CHECK_CUDA(cudaDeviceSynchronize());
   int v = 0;
   int rc = read_embed_status(&v, true);
-  if (rc || (rc = read_paged_cache_status(&v, true)) || (rc = read_paged_attn_status(&v, true)))
+  if (rc || (rc = read_paged_cache_status(&v, true)) || (rc = read_paged_attn_status(&v, true)) || (rc = read_paged_chunk_status(&v, true)))
     return rc;
   return clear_device_status_words();
 }

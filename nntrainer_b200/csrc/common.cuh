@@ -399,6 +399,7 @@ int launch_embedding(int qtype, const void *table, const float *ids, float *y, u
 int read_embed_status(int *out, bool clear);
 int read_paged_cache_status(int *out, bool clear);
 int read_paged_attn_status(int *out, bool clear);
+int read_paged_chunk_status(int *out, bool clear);
 int launch_paged_append(const nntr_paged_cache *c, const nntr_paged_batch *b, const float *q, const float *k, const float *v,
                         int64_t ld_q, int64_t ld_kv, const float *q_gamma, const float *k_gamma, float eps, const float *cos_tab,
                         const float *sin_tab, unsigned table_rows, void *q_out, int64_t ld_out, unsigned flags, cudaStream_t st);

@@ -12,7 +12,7 @@
  * that the small ones of a long context stay out of its subnormal numbers.
  */
 #include "cluster.cuh"
-#include "paged.cuh"
+#include "paged_attention.cuh"
 #include "pipeline.cuh"
 
 #include <algorithm>
@@ -31,16 +31,6 @@ int read_paged_attn_status(int *out, bool clear) {
   *out = v;
   return NNTR_CUDA_OK;
 }
-
-struct AttendArgs {
-  const void *q, *k, *v;
-  void *out;
-  const float *sink;
-  long long ld_q, ld_out;
-  int window, first; // window: INT_MAX / 2 where there is none
-  int out_f32;
-  float scale_log2; // log2(e) / sqrt(head_dim)
-};
 
 /* ------------------------------------------------------ a few query rows */
 
@@ -86,29 +76,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-/* Blocks of KEYS cache rows that hold what a tile of queries at positions lo .. hi sees: those of the first tokens, then the window's.
- * A row in none of the queries' sight counts as not there: it may hold anything. */
-struct Sight {
-  int lo, hi, window, first, from, head_blocks, first_block, blocks;
-  __device__ __forceinline__ Sight(int lo_, int hi_, int window_, int first_, int keys) : lo(lo_), hi(hi_), window(window_) {
-    from = max(0, lo - window + 1);
-    first = min(first_, from);
-    head_blocks = (first + keys - 1) / keys;
-    first_block = from / keys;
-    if (first_block <= head_blocks)
-      head_blocks = first_block = 0;
-    blocks = hi < 0 ? 0 : head_blocks + hi / keys - first_block + 1;
-  }
-  __device__ __forceinline__ int block(int i) const { return i < head_blocks ? i : i - head_blocks + first_block; }
-  __device__ __forceinline__ bool row_read(int j) const { return j <= hi && (j >= from || j < first); } // by one query at least
-};
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(AttendArgs a, PagedGeom g, PagedBatch s) {
   using Cfg = PdCfg<HD>;
@@ -298,7 +265,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
   auto store = [&](int row, int col, const float4 &sum, float mx, float total) {
     const int flat = tile * 16 + row, head = h * G + flat % G;
     if (a.sink && mx > -INFINITY)
-      total += ex2(a.sink[head] * 1.4426950408889634f - (mx - LIFT));
+      total += ex2(a.sink[head] * LOG2E - (mx - LIFT));
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const float4 f = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
     const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd + col;
@@ -390,7 +357,9 @@ int launch_paged_attention(const nntr_paged_cache *c, const nntr_paged_batch *b,
     return set_error(NNTR_CUDA_ERR_INVALID, "paged_attention: a window of no rows");
   constexpr int NONE = 0x3fffffff;
   AttendArgs a = {q, c->kcache, c->vcache, out, sink, ld_q, ld_out, (int)std::min(window, (unsigned)NONE),
-                  (int)std::min(first_tokens, (unsigned)NONE), out_dtype == NNTR_F32, 1.4426950408889634f / sqrtf((float)g.hd)};
+                  (int)std::min(first_tokens, (unsigned)NONE), out_dtype == NNTR_F32, LOG2E / sqrtf((float)g.hd)};
+  if (s.max_new * (g.hq / g.hkv) > 16)
+    return launch_paged_attention_chunk(a, c->dtype, g, s, b->max_rows, flags, st);
   const int G = g.hq / g.hkv, tiles = (int)(((long long)s.max_new * G + 15) / 16);
   const long long items = (long long)tiles * g.hkv * s.batch;
   long long seen = std::min<long long>((long long)a.window + a.first + s.max_new, b->max_rows ? b->max_rows : NONE);

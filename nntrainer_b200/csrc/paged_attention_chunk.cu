@@ -1,0 +1,567 @@
+// SPDX-License-Identifier: Apache-2.0
+/**
+ * @file  paged_attention_chunk.cu
+ * @brief Attention of chunks of new tokens over a key/value cache in pages, on the tensor cores (tcgen05, kind::f16).
+ *
+ * The formulas are those of paged_attention.cu. A tile is 128 rows of (token, query head of one kv head's group); a CTA holds two of
+ * them against the same cache rows, in steps of 128:
+ *   warps 0-3, 4-7  a thread per row of the first / second tile: S from tensor memory, running maximum, probabilities back to tensor
+ *                   memory over S as the next product's 16-bit operand, their sum. O is multiplied in place only when a row's maximum has grown by
+ *                   more than 2^7 since it was last done: until then the probabilities are that much larger, which their 16-bit type holds
+ *                   (fp16: 2^8 to keep small ones out of the subnormal numbers, times 2^7).
+ *   warp 8          one thread issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as it lies,
+ *                   dimensions contiguous). While one tile's probabilities are computed the other tile's products run.
+ *   warp 9          TMA copies of K and V tiles through one ring of slots: a box per page (128 rows of it at most) and 64 dimensions.
+ * Tensor memory: S (P) 128 columns a tile, O head_dim columns a tile. A step's products take 4 * 128 * 128 * head_dim flop a tile, its 16384
+ * exponentials as many clocks (16 a clock and SM) as its products at head_dim 128.
+ * Few tiles: the CTAs of a cluster share a pair of tiles along the cache rows and join through each other's shared memory.
+ * Every wait is bounded (pipeline.cuh).
+ */
+#include "cluster.cuh"
+#include "paged_attention.cuh"
+#include "pipeline.cuh"
+#include "tma_map.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace nntr {
+
+__device__ int g_paged_chunk_status = 0;
+
+int read_paged_chunk_status(int *out, bool clear) {
+  int v = 0;
+  NNTR_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_paged_chunk_status, sizeof(int)));
+  if (v && clear) {
+    const int zero = 0;
+    NNTR_CHECK_CUDA(cudaMemcpyToSymbol(g_paged_chunk_status, &zero, sizeof(int)));
+  }
+  *out = v;
+  return NNTR_CUDA_OK;
+}
+
+namespace {
+
+constexpr int PC_ROWS = 128; // of a tile: the MMA's M, lanes of tensor memory
+constexpr int PC_KEYS = 128; // cache rows of a step
+constexpr int PC_MMA_WARP = 8, PC_COPY_WARP = 9, PC_THREADS = 320;
+constexpr float PC_LIFT = 8.f, PC_GROWTH = 7.f; // log2
+constexpr uint32_t PC_POLLS = 1u << 22;
+template <int HD> struct PcCfg {
+  static constexpr int TILE = 128 * HD * 2; // bytes of a tile of Q, K or V: [64 dimensions of HD][row][128 B], 128-byte swizzle
+  static constexpr int SLOTS = HD == 128 ? 5 : 8;
+  static constexpr int OFF_RING = 2 * TILE;
+  static constexpr int OFF_BARS = OFF_RING + SLOTS * TILE;
+  static constexpr int SMEM = OFF_BARS + 256 + 1024; // the tiles begin at a multiple of 1024
+  // a CTA's part of a shared pair of tiles, in the tiles' place
+  static constexpr int PITCH = HD + 4; // floats of a row: neighbours' 16-byte pieces fall into different banks
+  static constexpr int OFF_ML = 2 * PC_ROWS * PITCH * 4;
+  static_assert(OFF_ML + 2 * PC_ROWS * 8 <= OFF_BARS && SMEM <= 227 * 1024, "shared memory of a CTA");
+};
+
+__device__ __forceinline__ bool pc_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+  return mbar_wait_warp(bar, parity, abort_flag, &g_paged_chunk_status, PC_POLLS, 2048);
+}
+
+/* shared-memory operand in 128-byte swizzled atoms of 8 rows; sbo: from 8 rows to the next 8, lbo: from 64 elements of a row to the next
+ * (used where the rows are the K dimension) */
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)((lbo >> 4) & 0x3fff) << 16) | ((uint64_t)((sbo >> 4) & 0x3fff) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+                 "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+                 "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+               "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_box4(uint32_t dst, const CUtensorMap *map, int x, int row, int head, int page, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(bar)
+               : "memory");
+}
+
+template <typename T> struct MmaType;
+template <> struct MmaType<__half> {
+  static constexpr uint32_t bits = 0;
+};
+template <> struct MmaType<__nv_bfloat16> {
+  static constexpr uint32_t bits = 1u << 7 | 1u << 10;
+};
+
+/* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. */
+__device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, int lane, int *seq, int *tile) {
+  int before = 0;
+  for (int b0 = 0; b0 < s.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b < s.batch ? (seq_rows(s, b).n * G + 2 * PC_ROWS - 1) / (2 * PC_ROWS) : 0;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(FULL, upto, o);
+      upto += lane >= o ? v : 0;
+    }
+    const unsigned m = __ballot_sync(FULL, before + upto > work);
+    if (m) {
+      const int l = __ffs(m) - 1;
+      *seq = b0 + l;
+      *tile = work - before - __shfl_sync(FULL, upto - n, l);
+      return true;
+    }
+    before += __shfl_sync(FULL, upto, 31);
+  }
+  return false;
+}
+
+} // namespace
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PC_THREADS, 1)
+paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttendArgs a, PagedGeom g,
+                             PagedBatch s) {
+  using Cfg = PcCfg<HD>;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t *smem = smem_raw + (sbase - smem_u32(smem_raw));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t bar0 = sbase + Cfg::OFF_BARS;
+  // slots full and empty; Q here; of a tile: S complete, P complete, O complete
+  auto FULL_BAR = [&](int i) { return bar0 + 8u * i; };
+  auto EMPTY_BAR = [&](int i) { return bar0 + 8u * (8 + i); };
+  const uint32_t Q_BAR = bar0 + 8 * 16;
+  auto S_BAR = [&](int t) { return bar0 + 8u * (17 + t); };
+  auto P_BAR = [&](int t) { return bar0 + 8u * (19 + t); };
+  auto O_BAR = [&](int t) { return bar0 + 8u * (21 + t); };
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Cfg::OFF_BARS + 192);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Cfg::OFF_BARS + 200);
+
+  if (tid == 0) {
+    for (int i = 0; i < Cfg::SLOTS; ++i) {
+      mbar_init(FULL_BAR(i), 1);
+      mbar_init(EMPTY_BAR(i), 1);
+    }
+    mbar_init(Q_BAR, 8);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(S_BAR(t), 1);
+      mbar_init(P_BAR(t), 4);
+      mbar_init(O_BAR(t), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == PC_MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto S_COL = [&](int t) { return tmem + 128u * t; };
+  auto O_COL = [&](int t) { return tmem + 256u + (uint32_t)HD * t; };
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const int parts = cluster_size(), part = cluster_rank(), G = g.hq / g.hkv, h = blockIdx.y;
+  int seq = 0, tile = 0;
+  const bool any = find_pair(s, G, blockIdx.x / parts, lane, &seq, &tile); // the same in every CTA of a cluster
+  SeqRows r = {};
+  if (any)
+    r = seq_rows(s, seq);
+  const int flat0 = tile * 2 * PC_ROWS, rows = any ? min(2 * PC_ROWS, r.n * G - flat0) : 0;
+  const bool two = rows > PC_ROWS;
+  const Sight sight(r.pos + flat0 / G, any ? r.pos + (flat0 + rows - 1) / G : -1, a.window, a.first, PC_KEYS);
+  const int b_lo = (int)((long long)sight.blocks * part / parts), steps = (int)((long long)sight.blocks * (part + 1) / parts) - b_lo;
+
+  if (warp < 8) {
+    /* ------------------------------ a thread per row ------------------------------ */
+    const int t = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane, flat = flat0 + t * PC_ROWS + row;
+    const bool there = t * PC_ROWS + row < rows;
+    const int p = there ? r.pos + flat / G : -1;
+    constexpr int CH = HD / 8; // 16-byte pieces of a row
+#pragma unroll 4
+    for (int i = lane; i < 32 * CH; i += 32) {
+      const int rr = wrow + i / CH, c = i % CH, f = flat0 + t * PC_ROWS + rr;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (t * PC_ROWS + rr < rows && 8 * c < g.hd)
+        w = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (r.first + f / G) * a.ld_q + (size_t)(h * G + f % G) * g.hd + 8 * c);
+      sts128(sbase + t * Cfg::TILE + (c >> 3) * (PC_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), w.x, w.y, w.z, w.w);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0)
+      mbar_arrive(Q_BAR);
+
+    const uint32_t trow = (uint32_t)wrow << 16;
+    float m = -INFINITY, l = 0.f; // the maximum that the row's probabilities refer to, in powers of two; their sum
+    bool ok = true;
+    const bool mine = t == 0 ? rows > 0 : two;
+    for (int j = 0; mine && j < steps; ++j) {
+      if (!(ok = pc_wait(S_BAR(t), j & 1, abort_flag)))
+        break;
+      fence_after();
+      uint32_t sr[PC_KEYS];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        tmem_ld32(S_COL(t) + trow + 32 * c, sr + 32 * c);
+      tmem_wait_ld();
+      const int j0 = sight.block(b_lo + j) * PC_KEYS;
+      if (!(j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first))) {
+#pragma unroll
+        for (int i = 0; i < PC_KEYS; ++i) {
+          const int key = j0 + i;
+          if (!(key <= p && (key > p - a.window || key < a.first)))
+            sr[i] = 0xff800000u;
+        }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < PC_KEYS; ++i)
+        mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sr[i]));
+      const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      const bool grown = big > m + PC_GROWTH;
+      if (__any_sync(FULL, grown)) {
+        const float keep = grown ? ex2(m - big) : 1.f;
+        l *= keep;
+        if (grown)
+          m = big;
+        if (j > 0) { // the products so far are complete: S of this step was issued behind them
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(O_COL(t) + trow + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+            tmem_st32(O_COL(t) + trow + 32 * c, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m - PC_LIFT;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pr[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float p0 = ex2(__fmaf_rn(__uint_as_float(sr[64 * c + 2 * i]), a.scale_log2, -base));
+          const float p1 = ex2(__fmaf_rn(__uint_as_float(sr[64 * c + 2 * i + 1]), a.scale_log2, -base));
+          sum[(2 * i) & 3] += p0;
+          sum[(2 * i + 1) & 3] += p1;
+          pr[i] = pack2<T>(p0, p1);
+        }
+        tmem_st32(S_COL(t) + trow + 32 * c, pr);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(P_BAR(t));
+    }
+
+    /* ------------------------------ the row's result ------------------------------ */
+    if (mine && steps > 0 && ok)
+      ok = pc_wait(O_BAR(t), 0, abort_flag);
+    if (two && parts > 1 && steps > 0 && ok) // what follows is written where the other tile's products read
+      ok = pc_wait(O_BAR(1 - t), 0, abort_flag);
+    fence_after();
+    if (mine && ok) {
+      const int head = h * G + flat % G;
+      float inv = 1.f;
+      if (parts == 1) {
+        float total = l;
+        if (a.sink && m > -INFINITY && there)
+          total += ex2(a.sink[head] * LOG2E - (m - PC_LIFT));
+        inv = total == 0.f ? 0.f : 1.f / total;
+      }
+      const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd;
+      float *part_row = reinterpret_cast<float *>(smem) + (t * PC_ROWS + row) * Cfg::PITCH;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        if (steps > 0) {
+          tmem_ld32(O_COL(t) + trow + 32 * c, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            o[i] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          float f[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            f[k] = __uint_as_float(o[i + k]) * inv;
+          const int col = 32 * c + i;
+          if (parts > 1) {
+            *reinterpret_cast<float4 *>(part_row + col) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4 *>(part_row + col + 4) = make_float4(f[4], f[5], f[6], f[7]);
+          } else if (there && col < g.hd) {
+            if (a.out_f32) {
+              float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + e + col);
+              dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+              dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+            } else {
+              *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + e + col) =
+                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+            }
+          }
+        }
+      }
+      if (parts > 1)
+        *reinterpret_cast<float2 *>(smem + Cfg::OFF_ML + 8 * (t * PC_ROWS + row)) = make_float2(m, l);
+    }
+  } else if (warp == PC_MMA_WARP) {
+    /* ------------------------------ products ------------------------------ */
+    constexpr uint32_t IDESC = 1u << 4 | MmaType<T>::bits | (uint32_t)(PC_ROWS >> 4) << 24;
+    constexpr uint32_t IDESC_S = IDESC | (uint32_t)(PC_KEYS >> 3) << 17;
+    constexpr uint32_t IDESC_O = IDESC | (uint32_t)(HD >> 3) << 17 | 1u << 16; // B: its rows are the K dimension
+    auto slot_at = [&](int item) { return sbase + Cfg::OFF_RING + (item % Cfg::SLOTS) * Cfg::TILE; };
+    auto here = [&](int item) { return pc_wait(FULL_BAR(item % Cfg::SLOTS), item / Cfg::SLOTS & 1, abort_flag); };
+    auto scores = [&](int t, int item) {
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
+          mma_ss(S_COL(t), sw128_desc(sbase + t * Cfg::TILE + at, 0, 1024), sw128_desc(slot_at(item) + at, 0, 1024), IDESC_S, k != 0);
+        }
+        mma_commit(S_BAR(t));
+      }
+    };
+    auto refilled = [&](int item) { return item + Cfg::SLOTS < 2 * steps; }; // else nobody waits for the slot: no arrival may be on its way at the end
+    const int tiles = two ? 2 : 1;
+    bool ok = rows > 0 && steps > 0 && pc_wait(Q_BAR, 0, abort_flag) && here(0);
+    if (ok) {
+      fence_after();
+      for (int t = 0; t < tiles; ++t)
+        scores(t, 0);
+      if (lane == 0 && refilled(0))
+        mma_commit(EMPTY_BAR(0));
+    }
+    for (int j = 0; j < steps && ok; ++j) {
+      const int vi = 2 * j + 1, ki = 2 * j + 2;
+      if (!(ok = here(vi)))
+        break;
+      const int j0 = sight.block(b_lo + j) * PC_KEYS;
+      if (!(j0 + PC_KEYS - 1 <= sight.hi && (j0 >= sight.from || j0 + PC_KEYS <= sight.first))) {
+        // rows that nobody sees meet probabilities of zero: what they hold must be finite
+        for (int i = lane; i < PC_KEYS * (HD / 8); i += 32) {
+          const int rr = i >> 3 & (PC_KEYS - 1);
+          if (!sight.row_read(j0 + rr))
+            sts128(slot_at(vi) + 16 * i, 0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      if (j + 1 < steps && !(ok = here(ki)))
+        break;
+      for (int t = 0; t < tiles; ++t) {
+        if (!(ok = pc_wait(P_BAR(t), j & 1, abort_flag)))
+          break;
+        fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int k = 0; k < PC_KEYS / 16; ++k)
+            mma_ts(O_COL(t), S_COL(t) + 8 * k, sw128_desc(slot_at(vi) + k * 2048, 128 * 128, 1024), IDESC_O, j != 0 || k != 0);
+          if (j + 1 == steps)
+            mma_commit(O_BAR(t));
+        }
+        if (j + 1 < steps)
+          scores(t, ki);
+      }
+      if (ok && lane == 0) {
+        if (refilled(vi))
+          mma_commit(EMPTY_BAR(vi % Cfg::SLOTS));
+        if (refilled(ki))
+          mma_commit(EMPTY_BAR(ki % Cfg::SLOTS));
+      }
+    }
+    __syncwarp();
+  } else {
+    /* ------------------------------ copies ------------------------------ */
+    const int page_rows = 1 << g.page_shift, box = min(page_rows, PC_KEYS);
+    constexpr int HALVES = HD / 64;
+    const int boxes = PC_KEYS / box * HALVES, at_row = lane / HALVES * box, half = lane % HALVES;
+    int page = 0, row = 0;
+    for (int i = 0; rows > 0 && i < 2 * steps; ++i) {
+      if ((i & 1) == 0 && lane < boxes) { // pages of the step, the same for keys and values
+        const int at = sight.block(b_lo + i / 2) * PC_KEYS + at_row;
+        page = g.n_pages; // outside the map: the box is filled with zeros
+        row = at & (page_rows - 1);
+        if (at <= sight.hi) {
+          const int given = __ldg(s.table + (size_t)seq * s.ld_table + (at >> g.page_shift));
+          if ((unsigned)given < (unsigned)g.n_pages)
+            page = given;
+          else
+            atomicExch(&g_paged_chunk_status, NNTR_CUDA_ERR_INVALID);
+        }
+      }
+      const int slot = i % Cfg::SLOTS, use = i / Cfg::SLOTS;
+      if (use > 0 && !pc_wait(EMPTY_BAR(slot), (use - 1) & 1, abort_flag))
+        break;
+      if (lane == 0)
+        mbar_expect_tx(FULL_BAR(slot), Cfg::TILE);
+      __syncwarp();
+      if (lane < boxes)
+        tma_box4(sbase + Cfg::OFF_RING + slot * Cfg::TILE + half * (PC_KEYS * 128) + at_row * 128, i & 1 ? &vmap : &kmap, half * 64, row, h, page,
+                 FULL_BAR(slot));
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0) // one that has no rows has no CTA either
+      for (int b = lane; b < s.batch; b += 32)
+        if (seq_rows(s, b).bad)
+          atomicExch(&g_paged_chunk_status, NNTR_CUDA_ERR_INVALID);
+    __syncwarp();
+  }
+
+  /* ------------------------------ a shared pair of tiles ------------------------------ */
+  if (parts > 1) {
+    cluster_sync();
+    const uint32_t raised = neighbour_raised(smem_u32(const_cast<int *>(abort_flag)), lane);
+    if (warp < 8 && !__any_sync(FULL, raised)) {
+      for (int R = part + parts * warp; R < rows; R += parts * 8) {
+        const int flat = flat0 + R, head = h * G + flat % G, col = 4 * lane;
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < parts) {
+            uint32_t remote;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(sbase + Cfg::OFF_ML + 8 * R), "r"(k));
+            asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(ml[k].x), "=f"(ml[k].y) : "r"(remote) : "memory");
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (col < HD)
+              v[k] = ld_cluster4(sbase + 4 * (R * Cfg::PITCH + col), k);
+          }
+        float big = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < parts)
+            big = fmaxf(big, ml[k].x);
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        float total = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < parts) {
+            const float w = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - big);
+            total += w * ml[k].y;
+            f = make_float4(f.x + w * v[k].x, f.y + w * v[k].y, f.z + w * v[k].z, f.w + w * v[k].w);
+          }
+        if (a.sink && big > -INFINITY)
+          total += ex2(a.sink[head] * LOG2E - (big - PC_LIFT));
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd + col;
+        if (col < g.hd) {
+          if (a.out_f32)
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + e) = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+          else
+            *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + e) = make_uint2(pack2<T>(f.x * inv, f.y * inv), pack2<T>(f.z * inv, f.w * inv));
+        }
+      }
+    }
+    cluster_sync(); // nobody leaves while its part is read
+  }
+
+  /* on an abort copies and products in flight get time to land before the memory is released */
+  if (*abort_flag)
+    for (int i = 0; i < 1000; ++i)
+      __nanosleep(1000);
+  fence_before();
+  __syncthreads();
+  if (warp == PC_MMA_WARP)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+/* ------------------------------------------------------------------ launch */
+
+template <typename T, int HD>
+static int launch_chunk(const AttendArgs &a, const PagedGeom &g, const PagedBatch &s, unsigned max_rows, unsigned flags, cudaStream_t st) {
+  auto kernel = paged_attention_chunk_kernel<T, HD>;
+  constexpr int smem = PcCfg<HD>::SMEM;
+  static std::atomic<bool> set[64];
+  int dev = 0;
+  NNTR_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
+    NNTR_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev >= 0 && dev < 64)
+      set[dev].store(true, std::memory_order_release);
+  }
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const int rc = encode_map_pages(&maps[i], i ? a.v : a.k, g.hd, 1 << g.page_shift, g.hkv, g.n_pages, g.page_stride,
+                                    std::min(1 << g.page_shift, PC_KEYS));
+    if (rc)
+      return rc;
+  }
+  const int G = g.hq / g.hkv;
+  const long long pair = 2 * PC_ROWS;
+  // no sequence has more than max_new rows, and all together no more than `tokens`
+  const long long pairs = std::min(s.batch * (((long long)s.max_new * G + pair - 1) / pair), (long long)s.tokens * G / pair + s.batch);
+  const long long seen = std::min<long long>((long long)a.window + a.first + s.max_new, max_rows ? max_rows : s.table_rows);
+  const long long blocks = (seen + PC_KEYS - 1) / PC_KEYS;
+  int parts = 1;
+  while (parts < 8 && 2 * pairs * g.hkv * parts <= sm_count() && blocks >= 4 * parts)
+    parts *= 2;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = {};
+  cfg.attrs = attr;
+  if (parts > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = parts;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (flags & NNTR_CUDA_GEMV_PDL) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.gridDim = dim3((unsigned)(pairs * parts), (unsigned)g.hkv);
+  cfg.blockDim = dim3(PC_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], a, g, s);
+  count_launch();
+  return check_cuda(e, "paged_attention launch");
+}
+
+int launch_paged_attention_chunk(const AttendArgs &a, int dtype, const PagedGeom &g, const PagedBatch &s, unsigned max_rows, unsigned flags,
+                                 cudaStream_t st) {
+  if (dtype == NNTR_F16)
+    return g.hd <= 64 ? launch_chunk<__half, 64>(a, g, s, max_rows, flags, st) : launch_chunk<__half, 128>(a, g, s, max_rows, flags, st);
+  return g.hd <= 64 ? launch_chunk<__nv_bfloat16, 64>(a, g, s, max_rows, flags, st)
+                    : launch_chunk<__nv_bfloat16, 128>(a, g, s, max_rows, flags, st);
+}
+
+} // namespace nntr

@@ -11,11 +11,11 @@
 
 namespace nntr {
 
-int encode_map_2d(CUtensorMap *map, const void *base, unsigned elem_bytes, uint64_t width, uint64_t rows, uint64_t stride,
-                  unsigned box_width, unsigned box_rows, bool swizzle) {
-  typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static int encoder(EncodeTiled *out) {
   static std::atomic<EncodeTiled> encode{nullptr};
   EncodeTiled enc = encode.load(std::memory_order_acquire);
   if (!enc) {
@@ -27,6 +27,28 @@ int encode_map_2d(CUtensorMap *map, const void *base, unsigned elem_bytes, uint6
     enc = reinterpret_cast<EncodeTiled>(fn);
     encode.store(enc, std::memory_order_release);
   }
+  *out = enc;
+  return NNTR_CUDA_OK;
+}
+
+int encode_map_pages(CUtensorMap *map, const void *base, unsigned head_dim, unsigned page_rows, unsigned heads, unsigned pages,
+                     uint64_t page_stride, unsigned box_rows) {
+  EncodeTiled enc;
+  if (const int rc = encoder(&enc))
+    return rc;
+  const cuuint64_t dims[4] = {head_dim, page_rows, heads, pages}, strides[3] = {2ull * heads * head_dim, 2ull * head_dim, 2 * page_stride};
+  const cuuint32_t box[4] = {64, box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NNTR_CUDA_OK : set_error(NNTR_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+int encode_map_2d(CUtensorMap *map, const void *base, unsigned elem_bytes, uint64_t width, uint64_t rows, uint64_t stride,
+                  unsigned box_width, unsigned box_rows, bool swizzle) {
+  EncodeTiled enc;
+  if (const int rc = encoder(&enc))
+    return rc;
   struct Key { // compared as bytes: no padding
     const void *base;
     uint64_t width, rows, stride;

@@ -18,6 +18,12 @@ namespace nntr {
 int encode_map_2d(CUtensorMap *map, const void *base, unsigned elem_bytes, uint64_t width, uint64_t rows, uint64_t stride,
                   unsigned box_width, unsigned box_rows, bool swizzle);
 
+/** Map over a cache in pages of 16-bit elements, [page][row][head][head_dim] with page_stride elements from page to page, as (dimension, row
+ *  of the page, head, page); a copy takes 64 dimensions of box_rows rows, 128-byte swizzled; what lies outside is zeros. base 16-byte
+ *  aligned, head_dim and page_stride multiples of 8. */
+int encode_map_pages(CUtensorMap *map, const void *base, unsigned head_dim, unsigned page_rows, unsigned heads, unsigned pages,
+                     uint64_t page_stride, unsigned box_rows);
+
 /** Copies the box at element x, row y of the map into shared memory; its bytes are counted on the mbarrier. x * element size
  *  must be a multiple of 16 bytes. */
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {

@@ -29,9 +29,11 @@ namespace {
 
 constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32;
 constexpr int SP_MAX_PARTS = 8;
-constexpr int SP_LIST = 12288;             // logits that the list holds
-constexpr int SP_HEAD = 4096;              // logits that it is meant for, the greatest ones
-constexpr int SP_AROUND = 8000;            // ... and around a cut further down: three standard deviations of the estimate and more
+static_assert(SP_THREADS == 512, "a thread per bin, two per digit");
+constexpr int SP_LIST = 6144;              // logits that the list holds
+constexpr int SP_HEAD = 2048;              // logits that it is meant for, the greatest ones
+constexpr int SP_AROUND = 4400;            // ... and around a cut further down: three standard deviations of the estimate and more
+constexpr int SP_FEW = 128;                // tokens that are compared each with each
 constexpr int SP_BINS = 512;               // of the estimate, over 46 powers of two of the weight
 constexpr int SP_EVERY = 8;                // every eighth block of 128 logits is in it
 constexpr double SP_ONE = 17592186044416.0; // 2^44: 2^20 logits of the greatest weight stay in 64 bits
@@ -50,13 +52,14 @@ struct SampleArgs {
 };
 
 struct SampleShared {
+  unsigned long long w[SP_LIST], few_w[SP_FEW];
   float x[SP_LIST];
-  uint32_t i[SP_LIST];
-  uint32_t hist[2][2][256]; // of a digit: the sum of its tokens' weights in two words
+  uint32_t i[SP_LIST], few_o[SP_FEW], few_i[SP_FEW];
+  uint32_t hist[2][2][256]; // of a digit: the sum of its tokens' weights in two words; digit d at d % 8 * 32 + d / 8
   uint32_t bins[SP_BINS], all_bins[SP_BINS]; // of this CTA's part of the row, of the row
   unsigned long long sub[SP_MAX_PARTS * SP_WARPS], sum[SP_WARPS], before, at;
   float max_of[SP_MAX_PARTS], warp_max[SP_WARPS], min_x, from, upto;
-  uint32_t counts[SP_MAX_PARTS], above[SP_MAX_PARTS], count, n_above, digit, verdict;
+  uint32_t counts[SP_MAX_PARTS], above[SP_MAX_PARTS], count, n_above, digit, verdict, few;
 };
 
 /* bits that ascend with the value; 0 for what is never drawn: NaN and -inf */
@@ -71,33 +74,60 @@ __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_flo
 /* Weights of a row. 2^f on [-1/2, 1/2]: polynomial of the least greatest relative error (2^-28.9) with value 1 at 0. */
 struct Weigher {
   float mx, exact_from; // the greatest logit; from here up in double precision
+  bool fp32;            // others in fp32; else all in double precision
   double top, per_t;
-  float c_hi, c_lo; // log2(e) / T
+  float c_hi, c_lo, m_hi, m_lo; // log2(e) / T, and times the greatest logit, each as a sum of two
 
   __device__ __forceinline__ Weigher(float mx_, double t) : mx(mx_), top(mx_), per_t(1.0 / t) {
     exact_from = fmaxf((float)(top - SP_EXACT_NATS * t), -3.402823466e38f);
-    const double c = 1.4426950408889634 / t;
+    const double c = 1.4426950408889634 / t, m = c * top;
     c_hi = (float)c;
-    c_lo = isinf(c_hi) ? 0.f : (float)(c - (double)c_hi);
+    c_lo = (float)(c - (double)c_hi);
+    m_hi = (float)(rint(m * 8.0) * 0.125); // plus a small whole number it is exact
+    m_lo = (float)(m - (double)m_hi);
+    fp32 = fabs(m) < 1048576.0;
+    if (!fp32) { // it is not: few logits are that large against the temperature
+      c_hi = c_lo = m_hi = m_lo = 0.f;
+      exact_from = -3.402823466e38f;
+    }
   }
   __device__ __forceinline__ double exactly(float x) const { return x == mx ? 1.0 : x > -INFINITY ? exp(((double)x - top) * per_t) : 0.0; }
-  __device__ __forceinline__ unsigned long long in_fp32(float x) const {
-    const float d = x - mx;
-    const float e = fabsf(x) > fabsf(mx) ? (x - d) - mx : x - (d + mx); // what the difference was rounded by
-    const float y = d * c_hi;
-    if (!(y > -46.f))
-      return 0ull;
-    const float n = rintf(y), f = fmaf(d, c_hi, -n) + fmaf(d, c_lo, e * c_hi);
-    float q = 1.535336190840639e-4f;
-    q = fmaf(q, f, 1.3398874413974103e-3f);
-    q = fmaf(q, f, 9.618437357669995e-3f);
-    q = fmaf(q, f, 5.550332471126199e-2f);
-    q = fmaf(q, f, 2.4022647913628897e-1f);
-    q = fmaf(q, f, 6.931472028550653e-1f);
-    return (unsigned long long)__float2uint_rn(fmaf(q, f, 1.f) * 1073741824.f) << 14 >> (int)-n;
+  __device__ __forceinline__ unsigned long long exact_one(float x) const { return __double2ull_rn(exactly(x) * SP_ONE); }
+  /* two logits, sums of their weights' integers; two operations in one instruction where they are fp32 */
+  __device__ __forceinline__ void in_fp32(float x0, float x1, unsigned long long *w0, unsigned long long *w1) const {
+    constexpr float MAGIC = 12582912.f; // 1.5 * 2^23: the sum's low bits are the nearest whole number
+    float y0 = -m_hi, y1 = -m_hi, g0 = -m_lo, g1 = -m_lo;
+    fma2(y0, y1, x0, x1, c_hi, c_hi);
+    fma2(g0, g1, x0, x1, c_lo, c_lo);
+    const float2 t = add2(y0, y1, MAGIC, MAGIC), n = add2(t.x, t.y, -MAGIC, -MAGIC), s = add2(n.x, n.y, m_hi, m_hi);
+    float f0 = -s.x, f1 = -s.y;
+    fma2(f0, f1, x0, x1, c_hi, c_hi);
+    const float2 f = add2(f0, f1, g0, g1);
+    float q0 = 1.3398874413974103e-3f, q1 = q0, r0, r1;
+    fma2(q0, q1, 1.535336190840639e-4f, 1.535336190840639e-4f, f.x, f.y);
+    r0 = r1 = 9.618437357669995e-3f;
+    fma2(r0, r1, q0, q1, f.x, f.y);
+    q0 = q1 = 5.550332471126199e-2f;
+    fma2(q0, q1, r0, r1, f.x, f.y);
+    r0 = r1 = 2.4022647913628897e-1f;
+    fma2(r0, r1, q0, q1, f.x, f.y);
+    q0 = q1 = 6.931472028550653e-1f;
+    fma2(q0, q1, r0, r1, f.x, f.y);
+    r0 = r1 = 1.f;
+    fma2(r0, r1, q0, q1, f.x, f.y);
+    *w0 = y0 > -46.f ? fixed_of(r0, t.x) : 0ull;
+    *w1 = y1 > -46.f ? fixed_of(r1, t.y) : 0ull;
+  }
+  static __device__ __forceinline__ unsigned long long fixed_of(float r, float t) { // r * 2^n * 2^44, n in t's low bits
+    const uint32_t b = __float_as_uint(r) + (__float_as_uint(t) << 23);
+    return (unsigned long long)((b & 0x7fffff) | 0x800000) << 21 >> (127 - (b >> 23));
   }
   __device__ __forceinline__ unsigned long long operator()(float x) const {
-    return x >= exact_from ? __double2ull_rn(exactly(x) * SP_ONE) : in_fp32(x);
+    if (x >= exact_from)
+      return exact_one(x);
+    unsigned long long w, same;
+    in_fp32(x, x, &w, &same);
+    return w;
   }
   /* the least logit with a weight of at least w, but no greater than the greatest */
   __device__ float least_with(double w) const {
@@ -169,18 +199,26 @@ __device__ uint32_t descend(SampleShared &sh, int parts, int bits, bool down, un
   int side = 0;
   for (int shift = (bits - 1) / 8 * 8; shift >= 0; shift -= 8, side ^= 1) {
     auto &h = sh.hist[side];
-    for (int i = tid; i < 2 * 256; i += SP_THREADS)
-      h[i >> 8][i & 255] = 0;
+    h[tid >> 8][tid & 255] = 0;
     __syncthreads();
-    each([&](uint32_t key, unsigned long long w) {
-      if ((unsigned long long)key >> (shift + 8) == prefix && w) {
-        const int d = key >> shift & 255;
-        const uint32_t add = (uint32_t)w, old = atomicAdd(&h[0][d], add), up = (uint32_t)(w >> 32) + (old + add < old);
-        if (up) // with the carry
-          atomicAdd(&h[1][d], up);
+    each([&](const uint32_t(&key)[4], const unsigned long long(&w)[4]) { // four on their way at a time
+      uint32_t old[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int d = key[k] >> shift & 255;
+        old[k] = 0;
+        if (w[k] && (unsigned long long)key[k] >> (shift + 8) == prefix)
+          old[k] = atomicAdd(&h[0][d % 8 * 32 + d / 8], (uint32_t)w[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int d = key[k] >> shift & 255;
+        const uint32_t up = (uint32_t)(w[k] >> 32) + (old[k] + (uint32_t)w[k] < old[k]); // with the carry
+        if (up && (unsigned long long)key[k] >> (shift + 8) == prefix)
+          atomicAdd(&h[1][d % 8 * 32 + d / 8], up);
       }
     });
-    if (parts > 1) { // the next level uses the other histogram: nobody writes into this one while it is read
+    if (parts > 1) {
       cluster_sync();
       unsigned long long all = 0;
       if (tid < 256)
@@ -195,23 +233,33 @@ __device__ uint32_t descend(SampleShared &sh, int parts, int bits, bool down, un
     __syncthreads();
     if (warp == 0) {
       unsigned long long v[8], run = 0;
+      const int column = down ? 31 - lane : lane; // eight digits
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int d = down ? 255 - (8 * lane + k) : 8 * lane + k;
-        v[k] = (unsigned long long)h[1][d] << 32 | h[0][d];
+        const int at8 = (down ? 7 - k : k) * 32 + column;
+        v[k] = (unsigned long long)h[1][at8] << 32 | h[0][at8];
         run += v[k];
       }
       const unsigned long long upto = warp_scan(run, lane) + sum, all = __shfl_sync(FULL, upto, 31);
       const unsigned long long goal = target < all ? target : all;
       const unsigned m = __ballot_sync(FULL, run > 0 && upto >= goal);
       if (m == 0 ? lane == 0 : lane == __ffs(m) - 1) {
-        unsigned long long in_front = upto - run;
-        int k = 0;
-        while (k < 7 && !(v[k] && in_front + v[k] >= goal))
-          in_front += v[k++];
-        sh.digit = down ? 255 - (8 * lane + k) : 8 * lane + k;
+        unsigned long long in_front = upto - run, here = 0;
+        int found = -1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (found < 0) {
+            if (v[k] && in_front + v[k] >= goal) {
+              found = k;
+              here = v[k];
+            } else {
+              in_front += v[k];
+            }
+          }
+        found = found < 0 ? 0 : found;
+        sh.digit = column * 8 + (down ? 7 - found : found);
         sh.before = in_front;
-        sh.at = v[k];
+        sh.at = here;
       }
     }
     __syncthreads();
@@ -220,13 +268,12 @@ __device__ uint32_t descend(SampleShared &sh, int parts, int bits, bool down, un
     *at = sh.at;
   }
   *before = sum;
-  __syncthreads();
   return prefix;
 }
 
 } // namespace
 
-__global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
   pdl_launch_dependents();
@@ -248,14 +295,18 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
   constexpr int AT = 4; // loads of a lane on their way at a time
   auto for_slice = [&](auto f) { // f(index, four logits); what is behind the slice is NaN
     for (unsigned i0 = s0 + 4 * lane; i0 - 4 * lane < s1; i0 += 128 * AT) {
-      float4 v[AT];
+      float v[AT][4];
 #pragma unroll
       for (int k = 0; k < AT; ++k) {
         const unsigned i = i0 + 128 * k;
-        if (a.vec && i + 4 <= s1)
-          v[k] = *reinterpret_cast<const float4 *>(x + i);
-        else
-          v[k] = make_float4(i < s1 ? x[i] : NAN, i + 1 < s1 ? x[i + 1] : NAN, i + 2 < s1 ? x[i + 2] : NAN, i + 3 < s1 ? x[i + 3] : NAN);
+        if (a.vec && i + 4 <= s1) {
+          const float4 w = *reinterpret_cast<const float4 *>(x + i);
+          v[k][0] = w.x, v[k][1] = w.y, v[k][2] = w.z, v[k][3] = w.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[k][e] = i + e < s1 ? x[i + e] : NAN;
+        }
       }
 #pragma unroll
       for (int k = 0; k < AT; ++k)
@@ -265,18 +316,17 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
 
   /* ---- the greatest logit */
   float mx = -INFINITY;
-  for_slice([&](unsigned, const float4 &v) { mx = fmaxf(fmaxf(mx, fmaxf(v.x, v.y)), fmaxf(v.z, v.w)); }); // a NaN never wins
+  for_slice([&](unsigned, const float(&v)[4]) { mx = fmaxf(fmaxf(mx, fmaxf(v[0], v[1])), fmaxf(v[2], v[3])); }); // a NaN never wins
 #pragma unroll
   for (int o = 16; o; o >>= 1)
     mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
   if (lane == 0)
     sh.warp_max[warp] = mx;
-  if (tid == 0)
-    sh.count = sh.verdict = 0;
   __syncthreads();
-  mx = sh.warp_max[0];
-  for (int i = 1; i < SP_WARPS; ++i)
-    mx = fmaxf(mx, sh.warp_max[i]);
+  mx = sh.warp_max[lane % SP_WARPS];
+#pragma unroll
+  for (int o = SP_WARPS / 2; o; o >>= 1)
+    mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
   if (parts > 1) {
     cluster_wait();
     if (tid < parts)
@@ -307,19 +357,18 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
   Weigher weight(mx, temperature);
   const bool has_k = top_k > 0 && top_k < a.n, has_p = top_p > 0.0 && top_p < 1.0;
   const bool whole = !has_k && !has_p && !(min_p > 0.0); // every token is kept
-  if (tid == 0)
+  if (tid == SP_THREADS - 1)
     sh.min_x = min_p > 0.0 ? weight.least_with(min_p) : -3.402823466e38f; // -inf is never kept
 
   /* ---- from which value up there are about SP_HEAD logits */
-  const float per_bin = weight.c_hi * (SP_BINS / 46.f);
+  const float per_bin = (float)(1.4426950408889634 * SP_BINS / 46.0 * weight.per_t);
   auto bin_of = [&](float v) { return min(SP_BINS - 1, (int)fminf((mx - v) * per_bin, (float)SP_BINS)); };
   auto edge_of = [&](int bin) { return bin >= SP_BINS ? -3.402823466e38f : mx - (float)bin / per_bin; }; // the least value of the bins in front
   float head = -3.402823466e38f;
   if (a.n > SP_LIST) {
     sh.bins[tid] = 0;
     __syncthreads();
-    const unsigned sub = part * SP_WARPS + warp;
-    for (unsigned i0 = s0 + sub % SP_EVERY * 128; i0 < s1; i0 += 128 * SP_EVERY)
+    for (unsigned i0 = s0 + (part * SP_WARPS + warp) % SP_EVERY * 128; i0 < s1; i0 += 128 * SP_EVERY)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const unsigned i = i0 + 32 * k + lane;
@@ -328,11 +377,13 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
           atomicAdd(&sh.bins[bin_of(v)], 1u);
       }
     __syncthreads();
-    if (parts > 1)
+    uint32_t all = sh.bins[tid];
+    if (parts > 1) {
       cluster_sync();
-    uint32_t all = 0;
-    for (int k = 0; k < parts; ++k)
-      all += parts > 1 ? ld_remote32(&sh.bins[tid], k) : sh.bins[tid];
+      all = 0;
+      for (int k = 0; k < parts; ++k)
+        all += ld_remote32(&sh.bins[tid], k);
+    }
     sh.all_bins[tid] = all;
     __syncthreads();
     if (warp == 0) { // the last bin that the counts so far, times SP_EVERY, are not too many with
@@ -354,14 +405,15 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
     }
     __syncthreads();
     head = sh.from;
-    weight.exact_from = fmaxf(weight.exact_from, head);
+    if (weight.fp32)
+      weight.exact_from = fmaxf(weight.exact_from, head);
   } else {
     __syncthreads();
   }
   const float min_x = sh.min_x;
 
-  /* Logits from `from` up to `below` into the list, which the first CTA gets; f(logit) for each of the others; what f adds up in each slice
-   * goes to sh.sub of the first CTA. Returns how many are listed, ~0 if they are too many. */
+  /* Logits from `from` up to `below` into the list, which the first CTA gets; the others, four at a time, to f(logits, for each whether it is
+   * in the list); what f adds up in each slice goes to sh.sub of the first CTA. Returns how many are listed, ~0 if they are too many. */
   unsigned long long slice_sum = 0;
   unsigned n_above = 0;
   auto gather = [&](float from, float below, auto f) {
@@ -370,24 +422,33 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
     slice_sum = 0;
     n_above = 0;
     __syncthreads();
-    for_slice([&](unsigned i, const float4 &v4) {
-      const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    for_slice([&](unsigned i, const float(&v)[4]) {
+      bool in[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool in = v[k] >= from && v[k] < below;
-        if (!in)
-          f(v[k]);
-        const unsigned m = __ballot_sync(FULL, in);
-        if (m) {
-          unsigned at = 0;
-          if (lane == 0)
-            at = atomicAdd(&sh.count, (unsigned)__popc(m));
-          at = __shfl_sync(FULL, at, 0) + __popc(m & ((1u << lane) - 1));
-          if (in && at < SP_LIST) {
-            sh.x[at] = v[k];
-            sh.i[at] = i + k;
-          }
+      for (int k = 0; k < 4; ++k)
+        in[k] = v[k] >= from && v[k] < below;
+      f(v, in);
+      if (__any_sync(FULL, in[0] || in[1] || in[2] || in[3])) {
+        const unsigned mine = in[0] + in[1] + in[2] + in[3];
+        unsigned upto = mine; // of the lanes so far
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const unsigned t = __shfl_up_sync(FULL, upto, o);
+          upto += lane >= o ? t : 0;
         }
+        unsigned at = 0;
+        if (lane == 31)
+          at = atomicAdd(&sh.count, upto);
+        at = __shfl_sync(FULL, at, 31) + upto - mine;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (in[k]) {
+            if (at < SP_LIST) {
+              sh.x[at] = v[k];
+              sh.i[at] = i + k;
+            }
+            ++at;
+          }
       }
     });
     slice_sum = warp_sum(slice_sum);
@@ -402,7 +463,6 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
         sh.sub[warp] = slice_sum;
       if (tid == 0)
         sh.above[0] = sh.n_above;
-      __syncthreads();
     } else {
       if (tid < parts) {
         st_remote32(&sh.counts[part], tid, own);
@@ -424,24 +484,37 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
         }
       cluster_sync();
     }
+    if (part == 0 && all <= SP_LIST) {
+      if (parts == 1)
+        __syncthreads();
+      for (unsigned i = tid; i < all; i += SP_THREADS)
+        sh.w[i] = weight(sh.x[i]);
+      __syncthreads();
+    }
     return all <= SP_LIST ? all : ~0u;
   };
 
   /* ---- the greatest logits listed, the others summed */
   const bool need_rest = whole || (has_p && !has_k);
-  unsigned listed = gather(head, INFINITY, [&](float v) {
-    if (v == INFINITY)
-      ++n_above;
-    else if (need_rest)
-      slice_sum += weight(v);
+  unsigned listed = gather(head, INFINITY, [&](const float(&v)[4], const bool(&in)[4]) {
+    if (!need_rest)
+      return;
+    unsigned long long w[4]; // what is not listed is below exact_from
+    weight.in_fp32(v[0], v[1], &w[0], &w[1]);
+    weight.in_fp32(v[2], v[3], &w[2], &w[3]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      slice_sum += in[k] ? 0 : w[k];
   });
-  const bool fits = listed != ~0u && mx < INFINITY; // an infinite logit is for the digits
+  const bool fits = listed != ~0u && weight.fp32; // else: by digits
+  const bool all_listed = head == -3.402823466e38f;
 
   // Does the list do? Where that shows in the first CTA only, the others wait for its word.
   bool by_list = fits && (whole || has_p || has_k || min_x >= head);
-  if (has_k && has_p && top_k > listed)
+  const bool deep_k = has_k && top_k > listed && !all_listed; // the top_k-th is not in it
+  if (deep_k && has_p)
     by_list = false;
-  const bool open = by_list && (has_k ? top_k > listed : has_p);
+  const bool open = by_list && (has_k ? deep_k : has_p);
   const double u = a.u[row];
   auto goal_of = [&](unsigned long long total) { // the first sum above u * total
     const unsigned long long t = u > 0.0 ? (unsigned long long)fmin(u * (double)total, (double)total) + 1 : 1;
@@ -449,25 +522,38 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
   };
   unsigned long long before, at;
 
+  uint32_t cut = 1, cut_idx = 0xffffffffu; // tokens above `cut` are kept, of those at it the ones with an index up to cut_idx
+  unsigned long long of_cut = 0;           // so many of those at the cut, the lowest indices; 0: no cut
+  auto kept = [&](unsigned i, float v) {
+    const uint32_t o = order_of(v);
+    return o && (!of_cut || o > cut || (o == cut && i <= cut_idx)) && (v >= min_x || v == mx);
+  };
+
   // The draw where it falls into a slice of the row: sh.sub holds the kept weights of the slices (in the first CTA).
-  auto draw_in_slices = [&](auto kept) {
+  auto draw_in_slices = [&] {
     const int n_sub = parts * SP_WARPS;
+    constexpr int EACH = SP_MAX_PARTS * SP_WARPS / 32;
     if (warp == 0) {
-      unsigned long long v[SP_MAX_PARTS * SP_WARPS / 32], run = 0;
+      unsigned long long v[EACH], run = 0;
 #pragma unroll
-      for (int k = 0; k < SP_MAX_PARTS * SP_WARPS / 32; ++k) {
-        const int i = lane * (SP_MAX_PARTS * SP_WARPS / 32) + k;
-        v[k] = i < n_sub ? sh.sub[i] : 0;
+      for (int k = 0; k < EACH; ++k) {
+        v[k] = lane * EACH + k < n_sub ? sh.sub[lane * EACH + k] : 0;
         run += v[k];
       }
       const unsigned long long upto = warp_scan(run, lane), total = __shfl_sync(FULL, upto, 31), goal = goal_of(total);
       const unsigned m = __ballot_sync(FULL, run > 0 && upto >= goal);
       if (lane == __ffs(m) - 1) {
         unsigned long long in_front = upto - run;
-        int k = 0;
-        while (k < SP_MAX_PARTS * SP_WARPS / 32 - 1 && !(v[k] && in_front + v[k] >= goal))
-          in_front += v[k++];
-        sh.digit = lane * (SP_MAX_PARTS * SP_WARPS / 32) + k;
+        int found = -1;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+          if (found < 0) {
+            if (v[k] && in_front + v[k] >= goal)
+              found = k;
+            else
+              in_front += v[k];
+          }
+        sh.digit = lane * EACH + found;
         sh.before = in_front;
         sh.at = total;
       }
@@ -501,23 +587,32 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
       }
   };
 
-  uint32_t cut = 1, cut_idx = 0xffffffffu; // tokens above `cut` are kept, of those at it the ones with an index up to cut_idx
-  unsigned long long of_cut = 0;           // so many of those at the cut, the lowest indices; 0: no cut
-  auto kept = [&](unsigned i, float v) {
-    const uint32_t o = order_of(v);
-    return o && (!of_cut || o > cut || (o == cut && i <= cut_idx)) && (v >= min_x || v == mx);
-  };
   // over the list (in the first CTA)
-  auto each = [&](bool count) {
-    return [&, count](auto f) {
-      for (unsigned i = tid; i < listed; i += SP_THREADS)
-        f(order_of(sh.x[i]), count ? 1ull : weight(sh.x[i]));
+  auto over_list = [&](auto key, auto w) { // for descend(): key(entry), w(entry)
+    return [&sh, listed, tid, key, w](auto f) {
+      for (unsigned i0 = tid; i0 < listed; i0 += 4 * SP_THREADS) {
+        uint32_t k4[4];
+        unsigned long long w4[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned i = i0 + k * SP_THREADS;
+          k4[k] = i < listed ? key(i) : 0;
+          w4[k] = i < listed ? w(i) : 0;
+        }
+        f(k4, w4);
+      }
     };
   };
+  // values by how far they lie below the greatest: fewer digits
+  const uint32_t best = order_of(mx);
+  auto depth = [&](unsigned i) { return best - order_of(sh.x[i]); };
+  auto bits_down_to = [&](float v) { return max(1, 32 - __clz(best - max(1u, order_of(v)))); };
+  const int index_bits = max(1, 32 - __clz(a.n - 1));
+  auto weight_of = [&](unsigned i) { return sh.w[i]; };
   auto list_sum = [&](auto which) {
     unsigned long long sum = 0;
     for (unsigned i = tid; i < listed; i += SP_THREADS)
-      sum += which(sh.i[i], sh.x[i]) ? weight(sh.x[i]) : 0;
+      sum += which(sh.i[i], sh.x[i]) ? sh.w[i] : 0;
     return cta_sum(sh, sum);
   };
   auto slices_sum = [&] {
@@ -532,8 +627,12 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
       of_cut = r;
     }
   };
-  auto cut_by_weight = [&](unsigned long long in_front, unsigned long long target) { // false: the list ends in front of the target
-    const uint32_t c = descend(sh, 1, 32, true, target - in_front, each(false), &before, &at);
+  auto cut_by_count = [&](float least, unsigned k) {
+    const uint32_t c = best - descend(sh, 1, bits_down_to(least), false, k, over_list(depth, [](unsigned) { return 1ull; }), &before, &at);
+    cut_at(c, k - before);
+  };
+  auto cut_by_weight = [&](float least, unsigned long long in_front, unsigned long long target) { // false: the list ends in front of the target
+    const uint32_t c = best - descend(sh, 1, bits_down_to(least), false, target - in_front, over_list(depth, weight_of), &before, &at);
     if (in_front + before + at < target)
       return false;
     const unsigned long long w = weight(value_of(c));
@@ -542,16 +641,68 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
   };
   auto place_cut = [&] { // which of the equal ones are kept
     if (of_cut)
-      cut_idx = descend(sh, 1, 20, false, of_cut, [&](auto f) {
-        for (unsigned i = tid; i < listed; i += SP_THREADS)
-          f(sh.i[i], order_of(sh.x[i]) == cut ? 1ull : 0ull);
-      }, &before, &at);
+      cut_idx = descend(sh, 1, index_bits, false, of_cut, over_list([&](unsigned i) { return sh.i[i]; }, [&](unsigned i) {
+        return order_of(sh.x[i]) == cut ? 1ull : 0ull;
+      }), &before, &at);
   };
   auto list_to_slices = [&] {
     for (unsigned i = tid; i < listed; i += SP_THREADS)
       if (kept(sh.i[i], sh.x[i]))
-        atomicAdd(&sh.sub[sh.i[i] / a.sub_len], weight(sh.x[i]));
+        atomicAdd(&sh.sub[sh.i[i] / a.sub_len], sh.w[i]);
     __syncthreads();
+  };
+  /* Where few tokens, no more than SP_FEW, lie above the cut and pass min_p (value `passes`): each is compared with each. all: the sum that top_p refers to (with top_k it
+   * is that of the tokens top_k leaves). False: there are more. */
+  auto among_few = [&](uint32_t passes, unsigned long long all) {
+    const uint32_t least = has_k && has_p ? cut : max(cut, passes); // that sum has the tokens too that min_p drops
+    if (tid == 0)
+      sh.few = 0;
+    __syncthreads();
+    for (unsigned i = tid; i < listed; i += SP_THREADS) {
+      const uint32_t o = order_of(sh.x[i]);
+      if (o >= least) {
+        const unsigned at = atomicAdd(&sh.few, 1u);
+        if (at < SP_FEW) {
+          sh.few_o[at] = o;
+          sh.few_i[at] = sh.i[i];
+          sh.few_w[at] = sh.w[i];
+        }
+      }
+    }
+    __syncthreads();
+    const int n = (int)sh.few;
+    if (n > SP_FEW)
+      return false;
+    const bool there = tid < n;
+    const uint32_t o = there ? sh.few_o[tid] : 0, id = there ? sh.few_i[tid] : 0;
+    const unsigned long long w = there ? sh.few_w[tid] : 0;
+    unsigned rank = 0;
+    unsigned long long in_front = 0;
+    if (warp * 32 < n)
+      for (int j = 0; j < n; ++j)
+        if (sh.few_o[j] > o || (sh.few_o[j] == o && sh.few_i[j] < id)) {
+          ++rank;
+          in_front += sh.few_w[j];
+        }
+    bool mine = there && (!has_k || rank < top_k);
+    if (has_p) {
+      if (has_k)
+        all = cta_sum(sh, mine ? w : 0);
+      mine = mine && in_front < (unsigned long long)ceil(top_p * (double)all);
+    }
+    mine = mine && o >= passes;
+    __syncthreads();
+    if (there)
+      sh.few_w[tid] = mine ? w : 0;
+    const unsigned long long total = cta_sum(sh, mine ? w : 0), goal = goal_of(total);
+    if (warp * 32 < n && __any_sync(FULL, mine)) {
+      unsigned long long upto = 0;
+      for (int j = 0; j < n; ++j)
+        upto += sh.few_i[j] <= id ? sh.few_w[j] : 0;
+      if (mine && w && upto >= goal && upto - w < goal)
+        tell(id, weight.exactly(value_of(o)) * SP_ONE / (double)total);
+    }
+    return true;
   };
   auto say = [&](unsigned word) { // the first CTA's word: 0 done, 1 one more pass from sh.from up to sh.upto, 2 by digits
     __syncthreads();
@@ -570,19 +721,32 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
   if (by_list && part == 0) {
     if (whole) {
       list_to_slices();
-      draw_in_slices([](unsigned, float) { return true; });
+      draw_in_slices();
       return;
     }
-    bool enough = !has_k || top_k <= listed;
-    if (has_k && top_k < listed) {
-      cut = descend(sh, 1, 32, true, top_k, each(true), &before, &at);
-      of_cut = top_k - before;
-    }
-    if (has_p && enough) {
-      unsigned long long sum = list_sum([&](unsigned, float v) { return !of_cut || order_of(v) > cut; });
-      sum += has_k ? of_cut * weight(value_of(cut)) : slices_sum();
+    const uint32_t least = min_x >= head ? order_of(min_x) : 1u; // what lies below fails min_p
+    bool enough = !deep_k;
+    if (has_k && top_k < listed)
+      cut_by_count(head, top_k);
+    unsigned long long sum = 0;
+    if (has_p && !has_k) {
+      sum = list_sum([](unsigned, float) { return true; }) + slices_sum();
       target = (unsigned long long)ceil(top_p * (double)sum);
-      enough = cut_by_weight(0, target);
+    }
+    bool done = false;
+    if (enough && (of_cut || least > 1u)) {
+      if (open && least > 1u)
+        say(0); // whatever top_p says, the kept tokens are listed
+      done = among_few(least, sum);
+    }
+    if (done)
+      return;
+    if (has_p && enough) {
+      if (has_k) {
+        sum = list_sum([&](unsigned, float v) { return !of_cut || order_of(v) > cut; }) + of_cut * weight(value_of(cut));
+        target = (unsigned long long)ceil(top_p * (double)sum);
+      }
+      enough = cut_by_weight(head, 0, target);
       if (!enough) { // about where it is: so much of the weight that is not listed lies in front of it
         const unsigned long long rest = slices_sum();
         if (warp == 0) {
@@ -602,29 +766,34 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
           const unsigned m = __ballot_sync(FULL, run > 0.0 && upto >= goal);
           if (lane == (m ? __ffs(m) - 1 : 31)) {
             double in_front = upto - run;
-            int k = 0;
-            while (k < SP_BINS / 32 - 1 && in_front + v[k] < goal)
-              in_front += v[k++];
-            sh.digit = lane * (SP_BINS / 32) + k;
+            int found = SP_BINS / 32;
+#pragma unroll
+            for (int k = 0; k < SP_BINS / 32; ++k)
+              if (found == SP_BINS / 32) {
+                if (in_front + v[k] >= goal)
+                  found = k;
+                else
+                  in_front += v[k];
+              }
+            sh.digit = min(SP_BINS - 1, lane * (SP_BINS / 32) + found);
           }
         }
       }
     } else if (!enough && warp == 0) { // top_k of more tokens than are listed
-      unsigned run = 0, v[SP_BINS / 32];
-#pragma unroll
+      unsigned run = 0;
       for (int k = 0; k < SP_BINS / 32; ++k)
-        run += v[k] = sh.all_bins[lane * (SP_BINS / 32) + k];
+        run += sh.all_bins[lane * (SP_BINS / 32) + k];
       const unsigned long long upto = warp_scan(run, lane);
       const unsigned m = __ballot_sync(FULL, run > 0 && upto * SP_EVERY >= top_k);
       if (lane == (m ? __ffs(m) - 1 : 31)) {
         unsigned long long in_front = upto - run;
         int k = 0;
-        while (k < SP_BINS / 32 - 1 && (in_front + v[k]) * SP_EVERY < top_k)
-          in_front += v[k++];
+        while (k < SP_BINS / 32 - 1 && (in_front + sh.all_bins[lane * (SP_BINS / 32) + k]) * SP_EVERY < top_k)
+          in_front += sh.all_bins[lane * (SP_BINS / 32) + k++];
         sh.digit = lane * (SP_BINS / 32) + k;
       }
     }
-    if (!enough && min_x >= head) // what passes min_p is listed, and in front of the cut
+    if (least > 1u) // what passes min_p is listed, and in front of any cut further down
       enough = true;
     __syncthreads();
     if (!enough && tid == 0) { // the bins around that one
@@ -638,15 +807,16 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
       sh.from = edge_of(lo);
     }
     word = enough ? 0 : 1;
-    if (open)
-      word = say(word);
+    if (open && !(least > 1u && !deep_k))
+      say(word);
     if (word == 0) {
+      if (of_cut && among_few(least, sum))
+        return;
       place_cut();
       const unsigned long long total = list_sum(kept);
-      const uint32_t id = descend(sh, 1, 20, false, goal_of(total), [&](auto f) {
-        for (unsigned i = tid; i < listed; i += SP_THREADS)
-          f(sh.i[i], kept(sh.i[i], sh.x[i]) ? weight(sh.x[i]) : 0);
-      }, &before, &at);
+      const uint32_t id = descend(sh, 1, index_bits, false, goal_of(total), over_list([&](unsigned i) { return sh.i[i]; }, [&](unsigned i) {
+        return kept(sh.i[i], sh.x[i]) ? sh.w[i] : 0;
+      }), &before, &at);
       if (tid == 0)
         tell(id, weight.exactly(x[id]) * SP_ONE / (double)total);
     }
@@ -661,11 +831,13 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
     /* ---- one more pass: the logits around the cut listed, those above summed */
     __syncthreads();
     const float from = sh.from, below = sh.upto;
-    listed = gather(from, below, [&](float v) {
-      if (v >= below) {
-        slice_sum += weight(v);
-        ++n_above;
-      }
+    listed = gather(from, below, [&](const float(&v)[4], const bool(&)[4]) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (v[k] >= below) {
+          slice_sum += weight(v[k]);
+          ++n_above;
+        }
     });
     word = listed == ~0u || min_x >= below ? 2 : 0;
     if (word == 0) {
@@ -676,19 +848,17 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
           for (int k = 0; k < parts; ++k)
             above += sh.above[k];
           found = above < top_k && top_k <= above + listed;
-          if (found) {
-            const uint32_t c = descend(sh, 1, 32, true, top_k - above, each(true), &before, &at);
-            cut_at(c, top_k - above - before);
-          }
+          if (found)
+            cut_by_count(from, top_k - above);
         } else {
           const unsigned long long above = slices_sum();
-          found = above < target && cut_by_weight(above, target);
+          found = above < target && cut_by_weight(from, above, target);
         }
         word = say(found ? 0 : 2);
         if (found) {
           place_cut();
           list_to_slices();
-          draw_in_slices(kept);
+          draw_in_slices();
         }
       } else {
         cluster_sync();
@@ -698,25 +868,29 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
     if (word == 0)
       return;
     cut = 1;
+    cut_idx = 0xffffffffu;
     of_cut = 0;
   }
 
   /* ---- the whole row by digits, every CTA its slices */
-  auto each_of_row = [&](bool count) {
-    return [&for_slice, &weight, count](auto f) {
-      for_slice([&](unsigned, const float4 &v4) {
-        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+  auto over_row = [&](auto key, auto w) { // key(index, logit), w(logit)
+    return [&, key, w](auto f) {
+      for_slice([&](unsigned i, const float(&v)[4]) {
+        uint32_t k4[4];
+        unsigned long long w4[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (const uint32_t o = order_of(v[k]))
-            f(o, count ? 1ull : weight(v[k]));
+        for (int k = 0; k < 4; ++k) {
+          k4[k] = key(i + k, v[k]);
+          w4[k] = order_of(v[k]) ? w(v[k]) : 0;
+        }
+        f(k4, w4);
       });
     };
   };
+  auto by_value = [](unsigned, float v) { return order_of(v); };
   auto weigh = [&](auto which) { // over the cluster; each slice's sum into every CTA
     unsigned long long sum = 0;
-    for_slice([&](unsigned i, const float4 &v4) {
-      const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    for_slice([&](unsigned i, const float(&v)[4]) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (which(i + k, v[k]))
@@ -732,43 +906,35 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a) {
         sh.sub[warp] = sum;
       __syncthreads();
     }
-    sum = 0;
-    for (int i = 0; i < parts * SP_WARPS; ++i)
-      sum += sh.sub[i];
-    return sum;
+    return slices_sum();
   };
+  __syncthreads();
   if (parts > 1)
     cluster_sync(); // the first CTA is through with its histograms
   if (has_k) {
-    cut = descend(sh, parts, 32, true, top_k, each_of_row(true), &before, &at);
+    cut = descend(sh, parts, 32, true, top_k, over_row(by_value, [](float) { return 1ull; }), &before, &at);
     of_cut = top_k - before < at ? top_k - before : at; // all of them where there are fewer tokens than top_k
   }
   if (has_p) {
-    const uint32_t above = cut;
-    const bool all = !has_k;
-    unsigned long long sum = weigh([&](unsigned, float v) { const uint32_t o = order_of(v); return all ? o != 0 : o > above; });
+    const uint32_t above = has_k ? cut : 0;
+    unsigned long long sum = weigh([&](unsigned, float v) { return order_of(v) > above; });
     if (has_k)
       sum += of_cut * weight(value_of(cut));
     if (parts > 1)
       cluster_sync(); // the sums are read before they are written again
     target = (unsigned long long)ceil(top_p * (double)sum);
-    const uint32_t c = descend(sh, parts, 32, true, target, each_of_row(false), &before, &at);
+    const uint32_t c = descend(sh, parts, 32, true, target, over_row(by_value, [&](float v) { return weight(v); }), &before, &at);
     const unsigned long long w = weight(value_of(c)), r = target > before && w ? (target - before + w - 1) / w : 1;
     cut_at(c, r);
   }
   if (of_cut)
-    cut_idx = descend(sh, parts, 20, false, of_cut, [&](auto f) {
-      for_slice([&](unsigned i, const float4 &v4) {
-        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (order_of(v[k]) == cut)
-            f(i + k, 1ull);
-      });
-    }, &before, &at);
+    cut_idx = descend(sh, parts, index_bits, false, of_cut, over_row([](unsigned i, float) { return i; }, [&](float v) {
+      return order_of(v) == cut ? 1ull : 0ull;
+    }), &before, &at);
+  __syncthreads();
   weigh(kept);
   if (part == 0)
-    draw_in_slices(kept);
+    draw_in_slices();
 }
 
 int launch_sample(const float *logits, int64_t rows, int64_t n, int64_t ld, const float *u, double temperature, unsigned top_k, double top_p,
@@ -793,7 +959,7 @@ int launch_sample(const float *logits, int64_t rows, int64_t n, int64_t ld, cons
       set[dev].store(true, std::memory_order_release);
   }
   int parts = 1;
-  while (parts < SP_MAX_PARTS && rows * parts < 2 * sm_count() && n >= 4ll * SP_THREADS * parts)
+  while (parts < SP_MAX_PARTS && rows * parts <= sm_count() && n >= 4ll * SP_THREADS * parts)
     parts *= 2;
   const unsigned per_warp = (unsigned)((n + parts * SP_WARPS - 1) / (parts * SP_WARPS));
   SampleArgs a = {logits, u, row_params, ld, (unsigned)n, (per_warp + 127) / 128 * 128, 0, temperature, top_p, min_p, top_k, idx, idx_f, prob};

@@ -12,6 +12,8 @@ libnntr_cuda.so. A missing library or device raises -- there is no CPU path.
 """
 from __future__ import annotations
 
+import struct as _struct
+
 import numpy as np
 
 from . import capi
@@ -576,49 +578,62 @@ class Attention:
 
 
 # ------------------------------------------- several sequences, a cache in pages
-def _on_device(*tensors) -> None:
-    """Kernels are launched on the current device, whose stream they are put into: the tensors have to lie there."""
-    here = None
+# A call costs little more than its launch: the checks below touch each tensor once or twice, and the structures of
+# include/nntr_cuda.h are packed in one go (native alignment, as the compiler lays them out).
+_PAGED_CACHE = _struct.Struct("@3Ii2Iq2Q")  # nntr_paged_cache
+_PAGED_BATCH = _struct.Struct("@5I3Q")  # nntr_paged_batch
+
+
+def _here(*tensors) -> None:
+    """Kernels are launched on the current device, into its stream: the tensors have to lie there. None passes."""
+    here = -2
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("a CUDA tensor is needed (there is no CPU path)")
-        if here is None:
+        if t is not None and t.get_device() != here:
+            if here != -2 or not t.is_cuda:
+                break
             here = _torch()._C._cuda_getDevice()
-        if t.get_device() != here:
-            raise ValueError(f"a tensor on cuda:{t.get_device()}, the current device is cuda:{here}")
+            if t.get_device() != here:
+                break
+    else:
+        return
+    raise ValueError(f"a tensor on {t.device}, the current device is {'none' if here == -2 else f'cuda:{here}'} (there is no CPU path)")
 
 
 def _typed(t, name: str, dtype, numel: int | None = None):
     """A dense array of that type; its address. None passes."""
     if t is None:
         return None
-    if t.dtype != dtype or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+    if t.dtype is not dtype or not t.is_contiguous() or (numel is not None and t.numel() != numel):
         raise ValueError(f"{name}: need a contiguous {dtype} tensor" + (f" of {numel} elements" if numel is not None else ""))
     return t.data_ptr()
 
 
-def _paged(kcache, vcache, n_heads_q: int, page_table, row_start, context, tokens: int, max_new: int, max_rows: int):
-    """The structures of a paged call from its tensors."""
-    torch = _torch()
-    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != vcache.dtype or kcache.stride() != vcache.stride():
+def _paged(torch, kcache, vcache, n_heads_q: int, page_table, row_start, context, tokens: int, max_new: int, max_rows: int):
+    """The structures of a paged call from its tensors, and the caches' type."""
+    shape, stride, t = kcache.shape, kcache.stride(), kcache.dtype
+    if len(shape) != 4 or vcache.shape != shape or vcache.dtype is not t or vcache.stride() != stride:
         raise ValueError("kcache and vcache: [n_pages, page_size, n_heads_kv, head_dim], alike in type and strides")
-    pages, ps, hkv, hd = kcache.shape
-    stride = kcache.stride()
+    pages, ps, hkv, hd = shape
     if stride[3] != 1 or stride[2] != hd or stride[1] != hkv * hd:
         raise ValueError("kcache and vcache: the rows of a page lie back to back")
-    dtype = {torch.float16: capi.F16, torch.bfloat16: capi.BF16}.get(kcache.dtype)
-    if dtype is None:
-        raise NotImplementedError(f"caches of fp16 or bf16 (got {kcache.dtype})")
-    batch = context.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != batch:
-        raise ValueError("page_table: [batch, pages of a sequence]")
-    c = capi.PagedCache(n_heads_q, hkv, hd, dtype, ps, pages, stride[0] if pages > 1 else 0, kcache.data_ptr(), vcache.data_ptr())
-    b = capi.PagedBatch(batch, tokens, max_new, max_rows, page_table.shape[1], _typed(row_start, "row_start", torch.int32, batch + 1),
-                        _typed(context, "context", torch.int32), _typed(page_table, "page_table", torch.int32))
-    from ctypes import byref
-    return byref(c), byref(b), dtype
+    if t is torch.float16:
+        dtype = capi.F16
+    elif t is torch.bfloat16:
+        dtype = capi.BF16
+    else:
+        raise NotImplementedError(f"caches of fp16 or bf16 (got {t})")
+    batch, table = context.numel(), page_table.shape
+    if len(table) != 2 or table[0] != batch or row_start.numel() != batch + 1:
+        raise ValueError("page_table: [batch, pages of a sequence]; row_start: one more than sequences")
+    i32 = torch.int32
+    if (page_table.dtype is not i32 or row_start.dtype is not i32 or context.dtype is not i32 or not page_table.is_contiguous()
+            or not row_start.is_contiguous() or not context.is_contiguous()):
+        raise ValueError("page_table, row_start and context: contiguous int32 tensors")
+    if min(max_new, max_rows) < 0:
+        raise ValueError("max_new and max_rows are counts")
+    return (_PAGED_CACHE.pack(n_heads_q, hkv, hd, dtype, ps, pages, stride[0] if pages > 1 else 0, kcache.data_ptr(), vcache.data_ptr()),
+            _PAGED_BATCH.pack(batch, tokens, max_new, max_rows, table[1], row_start.data_ptr(), context.data_ptr(), page_table.data_ptr()),
+            dtype)
 
 
 def paged_append(q, k, v, kcache, vcache, page_table, row_start, context, max_new: int, cos, sin, qk_norm=None, q_out=None,
@@ -628,26 +643,31 @@ def paged_append(q, k, v, kcache, vcache, page_table, row_start, context, max_ne
     [tokens, n_heads_q, head_dim]. q [tokens, n_heads_q * head_dim], k and v [tokens, n_heads_kv * head_dim]: fp32, rows may be slices of
     wider ones; cos, sin: device tables as ``rope_table`` makes them. The arrays of the batch: see ``paged_attention``."""
     torch = _torch()
-    hd, tokens = kcache.shape[-1], q.shape[0]
-    _on_device(q, k, v, kcache, vcache, page_table, row_start, context, cos, sin, q_out)
-    if q.dim() != 2 or k.shape != v.shape or k.dim() != 2 or k.shape[0] != tokens or k.shape[1] != kcache.shape[2] * hd or q.shape[1] % hd:
-        raise ValueError("q [tokens, n_heads_q * head_dim], k and v [tokens, n_heads_kv * head_dim]")
-    if q.dtype != torch.float32 or k.dtype != torch.float32 or v.dtype != torch.float32 or k.stride() != v.stride() or q.stride(1) != 1 or k.stride(1) != 1:
-        raise ValueError("q, k and v: fp32 rows; those of k and v at the same distance")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != hd:
-        raise ValueError("cos and sin: [positions, head_dim]")
-    hq = q.shape[1] // hd
-    c, b, _ = _paged(kcache, vcache, hq, page_table, row_start, context, tokens, max_new, 0)
-    if q_out is None:
-        q_out = torch.empty((tokens, hq, hd), dtype=kcache.dtype, device=q.device)
-    elif q_out.dtype != kcache.dtype or q_out.shape != (tokens, hq, hd) or q_out.stride(2) != 1 or q_out.stride(1) != hd:
-        raise ValueError("q_out: [tokens, n_heads_q, head_dim] in the caches' type")
     qg, kg, eps = qk_norm if qk_norm is not None else (None, None, 0.0)
-    _on_device(qg, kg)
-    check(lib().nntr_cuda_paged_append_dev(
-        c, b, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), _typed(qg, "q_gamma", torch.float32, hd),
-        _typed(kg, "k_gamma", torch.float32, hd), eps, _typed(cos, "cos", torch.float32), _typed(sin, "sin", torch.float32), cos.shape[0],
-        q_out.data_ptr(), q_out.stride(0), _flags(pdl), _stream()))
+    _here(q, k, v, kcache, vcache, page_table, row_start, context, cos, sin, q_out, qg, kg)
+    (tokens, width), f32, ld, ld_kv = q.shape, torch.float32, q.stride(), k.stride()
+    hkv, hd = kcache.shape[-2:]
+    kv_shape = k.shape
+    if v.shape != kv_shape or len(kv_shape) != 2 or kv_shape[0] != tokens or kv_shape[1] != hkv * hd or width % hd:
+        raise ValueError("q [tokens, n_heads_q * head_dim], k and v [tokens, n_heads_kv * head_dim]")
+    if q.dtype is not f32 or k.dtype is not f32 or v.dtype is not f32 or v.stride() != ld_kv or ld[1] != 1 or ld_kv[1] != 1:
+        raise ValueError("q, k and v: fp32 rows; those of k and v at the same distance")
+    rows = cos.shape
+    if len(rows) != 2 or sin.shape != rows or rows[1] != hd:
+        raise ValueError("cos and sin: [positions, head_dim]")
+    hq = width // hd
+    c, b, _ = _paged(torch, kcache, vcache, hq, page_table, row_start, context, tokens, max_new, 0)
+    if q_out is None:
+        q_out, ld_out = kcache.new_empty((tokens, hq, hd)), width
+    else:
+        ld_out, one, two = q_out.stride()
+        if q_out.dtype is not kcache.dtype or q_out.shape != (tokens, hq, hd) or two != 1 or one != hd:
+            raise ValueError("q_out: [tokens, n_heads_q, head_dim] in the caches' type")
+    rc = lib().nntr_cuda_paged_append_dev(
+        c, b, q.data_ptr(), k.data_ptr(), v.data_ptr(), ld[0], ld_kv[0], _typed(qg, "q_gamma", f32, hd), _typed(kg, "k_gamma", f32, hd), eps,
+        _typed(cos, "cos", f32), _typed(sin, "sin", f32), rows[0], q_out.data_ptr(), ld_out, capi.GEMV_PDL if pdl else 0, _stream())
+    if rc:
+        check(rc)
     return q_out
 
 
@@ -661,33 +681,46 @@ def paged_attention(q, kcache, vcache, page_table, row_start, context, max_new: 
     j < first_tokens; ``sink``: fp32 logits [n_heads_q]. ``out``: [tokens, n_heads_q, head_dim] in the caches' type (made if None) or
     fp32, the form the projections take; rows behind the last sequence are left as they are."""
     torch = _torch()
-    _on_device(q, kcache, vcache, page_table, row_start, context, sink, out)
-    if q.dim() != 3 or q.shape[2] != kcache.shape[-1] or q.dtype != kcache.dtype or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+    _here(q, kcache, vcache, page_table, row_start, context, sink, out)
+    (tokens, hq, hd), ld, t = q.shape, q.stride(), q.dtype
+    if hd != kcache.shape[-1] or t is not kcache.dtype or ld[2] != 1 or ld[1] != hd:
         raise ValueError("q: [tokens, n_heads_q, head_dim] in the caches' type")
-    tokens, hq, hd = q.shape
-    c, b, dtype = _paged(kcache, vcache, hq, page_table, row_start, context, tokens, max_new, max_rows)
+    c, b, dtype = _paged(torch, kcache, vcache, hq, page_table, row_start, context, tokens, max_new, max_rows)
+    if window is not None and window < 0 or first_tokens < 0:
+        raise ValueError("window and first_tokens are counts")
     if out is None:
-        out = torch.empty((tokens, hq, hd), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != hd or out.dtype not in (q.dtype, torch.float32):
-        raise ValueError("out: [tokens, n_heads_q, head_dim] in the caches' type or fp32")
-    check(lib().nntr_cuda_paged_attention_dev(
-        c, b, q.data_ptr(), q.stride(0), 0xFFFFFFFF if window is None else window, first_tokens, _typed(sink, "sink", torch.float32, hq),
-        out.data_ptr(), capi.F32 if out.dtype == torch.float32 else dtype, out.stride(0), _flags(pdl), _stream()))
+        out = q.new_empty((tokens, hq, hd))
+        ld_out = hq * hd
+    else:
+        ld_out, one, two = out.stride()
+        if out.shape != q.shape or two != 1 or one != hd or out.dtype not in (t, torch.float32):
+            raise ValueError("out: [tokens, n_heads_q, head_dim] in the caches' type or fp32")
+        dtype = capi.F32 if out.dtype is torch.float32 else dtype
+    rc = lib().nntr_cuda_paged_attention_dev(
+        c, b, q.data_ptr(), ld[0], 0xFFFFFFFF if window is None else window, first_tokens, _typed(sink, "sink", torch.float32, hq),
+        out.data_ptr(), dtype, ld_out, capi.GEMV_PDL if pdl else 0, _stream())
+    if rc:
+        check(rc)
     return out
 
 
 def copy_pages(caches, src, dst, pdl: bool = False) -> None:
     """Pages src[i] -> dst[i] in every array of ``caches`` ([..., n_pages, page_size, n_heads_kv, head_dim], contiguous: the key and
     value caches of all layers), in one launch. src and dst: int32 device tensors; no page twice in dst, or in both."""
-    torch = _torch()
-    _on_device(caches, src, dst)
-    if caches.dim() < 4 or not caches.is_contiguous():
+    i32 = _torch().int32
+    _here(caches, src, dst)
+    shape = caches.shape
+    if len(shape) < 4 or not caches.is_contiguous():
         raise ValueError("caches: a contiguous [..., n_pages, page_size, n_heads_kv, head_dim]")
-    n = src.numel()
-    page = caches.stride(-4) * caches.element_size()
-    pages = caches.shape[-4]
-    check(lib().nntr_cuda_copy_pages_dev(caches.data_ptr(), caches.numel() // (caches.stride(-4) * pages) if n else 0, page * pages, page, pages,
-                                         _typed(src, "src", torch.int32), _typed(dst, "dst", torch.int32, n), n, _flags(pdl), _stream()))
+    n, pages = src.numel(), shape[-4]
+    page = caches.element_size() * shape[-3] * shape[-2] * shape[-1]
+    arrays = 1
+    for d in shape[:-4]:
+        arrays *= d
+    rc = lib().nntr_cuda_copy_pages_dev(caches.data_ptr(), arrays, page * pages, page, pages, _typed(src, "src", i32), _typed(dst, "dst", i32, n), n,
+                                        capi.GEMV_PDL if pdl else 0, _stream())
+    if rc:
+        check(rc)
 
 
 def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, params=None, out=(None, None, None),
@@ -696,19 +729,28 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     top_k (0: off), top_p (1: off) and min_p (0: off), applied in that order (nntr_cuda_sample_dev). ``params``: fp32 [rows, 4] of the four for
     each row instead. Returns (uint32 indices as an int32 tensor, the same as float32, the tokens' probabilities among the kept)."""
     torch = _torch()
-    _on_device(logits, u, params)
-    n = logits.shape[-1]
-    if logits.dtype != torch.float32 or logits.stride(-1) != 1 or (logits.dim() > 2 and not logits.is_contiguous()):
+    f32 = torch.float32
+    idx, idx_f, prob = out
+    _here(logits, u, params, idx, idx_f, prob)
+    shape, stride = logits.shape, logits.stride()
+    n = shape[-1]
+    if logits.dtype is not f32 or stride[-1] != 1 or (len(shape) > 2 and not logits.is_contiguous()):
         raise ValueError("logits: fp32 [rows, n]")
+    if top_k < 0:
+        raise ValueError("top_k is a count")
     rows = logits.numel() // n if n else 0
-    ld = logits.stride(0) if logits.dim() == 2 else n
-    new = lambda t, dt: torch.empty(rows, dtype=dt, device=logits.device) if t is None else t  # noqa: E731
-    idx, idx_f, prob = new(out[0], torch.int32), new(out[1], torch.float32), new(out[2], torch.float32)
-    _on_device(idx, idx_f, prob)
-    check(lib().nntr_cuda_sample_dev(
-        logits.data_ptr(), rows, n, ld, _typed(u, "u", torch.float32, rows), temperature, top_k, top_p, min_p,
-        _typed(params, "params", torch.float32, 4 * rows), _typed(idx, "out", torch.int32, rows), _typed(idx_f, "out", torch.float32, rows),
-        _typed(prob, "out", torch.float32, rows), _flags(pdl), _stream()))
+    if idx is None and idx_f is None and prob is None:  # one allocation
+        idx, idx_f, prob = torch.empty((3, rows), dtype=f32, device=logits.device).unbind()
+        idx = idx.view(torch.int32)
+    else:
+        new = lambda t, dt: torch.empty(rows, dtype=dt, device=logits.device) if t is None else t  # noqa: E731
+        idx, idx_f, prob = new(idx, torch.int32), new(idx_f, f32), new(prob, f32)
+    rc = lib().nntr_cuda_sample_dev(
+        logits.data_ptr(), rows, n, stride[0] if len(shape) == 2 else n, _typed(u, "u", f32, rows), temperature, top_k, top_p, min_p,
+        _typed(params, "params", f32, 4 * rows), _typed(idx, "out", torch.int32, rows), _typed(idx_f, "out", f32, rows),
+        _typed(prob, "out", f32, rows), capi.GEMV_PDL if pdl else 0, _stream())
+    if rc:
+        check(rc)
     return idx, idx_f, prob
 
 

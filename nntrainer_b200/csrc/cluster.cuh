@@ -94,6 +94,22 @@ cudaError_t launch_in_clusters(void (*kernel)(P...), dim3 grid, int parts, int t
   return cudaLaunchKernelEx(&cfg, kernel, (P)args...);
 }
 
+/** Lets a kernel have more dynamic shared memory than the default, per device, once. */
+struct SmemOptIn {
+  std::atomic<bool> done[64];
+
+  template <typename... P> int operator()(void (*kernel)(P...), int smem) {
+    int dev = 0;
+    NNTR_CHECK_CUDA(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire))
+      return NNTR_CUDA_OK;
+    NNTR_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev >= 0 && dev < 64)
+      done[dev].store(true, std::memory_order_release);
+    return NNTR_CUDA_OK;
+  }
+};
+
 /** Clusters of 2, 4 or 8 CTAs of one kernel that run at the same time, per device, asked for once. */
 struct ClusterFit {
   std::atomic<int> n[64][3];

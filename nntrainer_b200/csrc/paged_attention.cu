@@ -310,7 +310,9 @@ template <typename T, int HD>
 static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch &s, int parts, int tiles, unsigned flags, cudaStream_t st) {
   auto kernel = paged_attention_few_kernel<T, HD>;
   constexpr int smem = PdCfg<HD>::SMEM;
-  NNTR_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static SmemOptIn opt_in;
+  if (const int rc = opt_in(kernel, smem))
+    return rc;
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.attrs = attr;

@@ -23,7 +23,6 @@
 #include "tma_map.cuh"
 
 #include <algorithm>
-#include <atomic>
 
 namespace nntr {
 
@@ -509,14 +508,9 @@ template <typename T, int HD>
 static int launch_chunk(const AttendArgs &a, const PagedGeom &g, const PagedBatch &s, unsigned max_rows, unsigned flags, cudaStream_t st) {
   auto kernel = paged_attention_chunk_kernel<T, HD>;
   constexpr int smem = PcCfg<HD>::SMEM;
-  static std::atomic<bool> set[64];
-  int dev = 0;
-  NNTR_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
-    NNTR_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (dev >= 0 && dev < 64)
-      set[dev].store(true, std::memory_order_release);
-  }
+  static SmemOptIn opt_in;
+  if (const int rc = opt_in(kernel, smem))
+    return rc;
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
     const int rc = encode_map_pages(&maps[i], i ? a.v : a.k, g.hd, 1 << g.page_shift, g.hkv, g.n_pages, g.page_stride,

@@ -21,7 +21,6 @@
 #include "pipeline.cuh"
 
 #include <algorithm>
-#include <atomic>
 
 namespace nntr {
 
@@ -950,14 +949,9 @@ int launch_sample(const float *logits, int64_t rows, int64_t n, int64_t ld, cons
     return set_error(NNTR_CUDA_ERR_INVALID, "sample: temperature %g, top_p %g, min_p %g; need temperature from 0 to 1e30, top_p >= 0, min_p from 0 to 1",
                      temperature, top_p, min_p);
   constexpr int smem = sizeof(SampleShared);
-  static std::atomic<bool> set[64];
-  int dev = 0;
-  NNTR_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
-    NNTR_CHECK_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (dev >= 0 && dev < 64)
-      set[dev].store(true, std::memory_order_release);
-  }
+  static SmemOptIn opt_in;
+  if (const int rc = opt_in(sample_kernel, smem))
+    return rc;
   int parts = 1;
   while (parts < SP_MAX_PARTS && rows * parts <= sm_count() && n >= 4ll * SP_THREADS * parts)
     parts *= 2;

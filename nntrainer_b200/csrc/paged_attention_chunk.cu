@@ -43,7 +43,9 @@ namespace {
 
 constexpr int PC_ROWS = 128; // of a tile: the MMA's M, lanes of tensor memory
 constexpr int PC_KEYS = 128; // cache rows of a step
-constexpr int PC_MMA_WARP = 8, PC_COPY_WARP = 9, PC_THREADS = 320;
+constexpr int PC_MMA_WARP = 8, PC_COPY_WARP = 9, PC_THREADS = 384; // warps 10 and 11 only make the third group of four whole
+/* Registers of a thread: 168 at launch (384 * 168 of the 65536); the third group gives some to the others: 2 * 208 + 88 = 3 * 168. */
+constexpr int PC_REGS_ROWS = 208, PC_REGS_REST = 88;
 constexpr float PC_LIFT = 8.f, PC_GROWTH = 7.f; // log2
 constexpr uint32_t PC_POLLS = 1u << 22;
 template <int HD> struct PcCfg {
@@ -116,6 +118,54 @@ template <> struct MmaType<__half> {
 template <> struct MmaType<__nv_bfloat16> {
   static constexpr uint32_t bits = 1u << 7 | 1u << 10;
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+/* 2^x of two numbers from -126 up, x below 16, on the FMA pipes: x = n + f with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f
+ * by the polynomial of the least greatest relative error with value 1 at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2),
+ * n into the exponent. */
+template <typename T> __device__ __forceinline__ float2 ex2_fma(float2 x) {
+  constexpr float MAGIC = 12582912.f;
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = add2(x.x, x.y, MAGIC, MAGIC), n = add2(t.x, t.y, -MAGIC, -MAGIC), f = add2(x.x, x.y, -n.x, -n.y);
+  float2 p;
+  if constexpr (sizeof(T) == 2 && MmaType<T>::bits == 0) {
+    p = make_float2(5.590642467794357e-2f, 5.590642467794357e-2f);
+    fma2(p.x, p.y, f.x, f.y, 9.582853038422538e-3f, 9.582853038422538e-3f);
+    float2 q = make_float2(2.4024098611601802e-1f, 2.4024098611601802e-1f);
+    fma2(q.x, q.y, p.x, p.y, f.x, f.y);
+    p = make_float2(6.931241934031505e-1f, 6.931241934031505e-1f);
+    fma2(p.x, p.y, q.x, q.y, f.x, f.y);
+  } else {
+    float2 q = make_float2(2.422109594702074e-1f, 2.422109594702074e-1f);
+    fma2(q.x, q.y, f.x, f.y, 5.5008930492411165e-2f, 5.5008930492411165e-2f);
+    p = make_float2(6.932829272228233e-1f, 6.932829272228233e-1f);
+    fma2(p.x, p.y, q.x, q.y, f.x, f.y);
+  }
+  float2 r = make_float2(1.f, 1.f);
+  fma2(r.x, r.y, p.x, p.y, f.x, f.y);
+  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
+}
+
+/* 64 scores of a row to probabilities 2^(s * scale - base), packed, and their sum. ALL: none is masked; then PC_BY_FMA of every eight pairs
+ * are computed beside the special function unit, which alone would take as many clocks as a step's products. */
+constexpr int PC_BY_FMA = 3;
+template <typename T, bool ALL>
+__device__ __forceinline__ void weights64(const uint32_t *s, float scale, float base, uint32_t *p, float2 (&sum)[2]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    float2 x = make_float2(-base, -base);
+    fma2(x.x, x.y, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), scale, scale);
+    x = ALL && i % 8 < PC_BY_FMA ? ex2_fma<T>(x) : make_float2(ex2(x.x), ex2(x.y));
+    sum[i & 1] = add2(sum[i & 1].x, sum[i & 1].y, x.x, x.y);
+    p[i] = pack2<T>(x.x, x.y);
+  }
+}
 
 /* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. */
 __device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, int lane, int *seq, int *tile) {
@@ -201,7 +251,10 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   const Sight sight(r.pos + flat0 / G, any ? r.pos + (flat0 + rows - 1) / G : -1, a.window, a.first, PC_KEYS);
   const int b_lo = (int)((long long)sight.blocks * part / parts), steps = (int)((long long)sight.blocks * (part + 1) / parts) - b_lo;
 
+  if (warp >= 8)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PC_REGS_REST));
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PC_REGS_ROWS));
     /* ------------------------------ a thread per row ------------------------------ */
     const int t = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane, flat = flat0 + t * PC_ROWS + row;
     const bool there = t * PC_ROWS + row < rows;
@@ -234,7 +287,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         tmem_ld32(S_COL(t) + trow + 32 * c, sr + 32 * c);
       tmem_wait_ld();
       const int j0 = sight.block(b_lo + j) * PC_KEYS;
-      if (!(j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first))) {
+      const bool all = j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first);
+      if (!all) {
 #pragma unroll
         for (int i = 0; i < PC_KEYS; ++i) {
           const int key = j0 + i;
@@ -244,9 +298,9 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < PC_KEYS; ++i)
-        mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sr[i]));
-      const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      for (int i = 0; i < PC_KEYS; i += 2)
+        mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+      const float big = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
       const bool grown = big > m + PC_GROWTH;
       if (__any_sync(FULL, grown)) {
         const float keep = grown ? ex2(m - big) : 1.f;
@@ -267,21 +321,17 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         }
       }
       const float base = m == -INFINITY ? 0.f : m - PC_LIFT;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t pr[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float p0 = ex2(__fmaf_rn(__uint_as_float(sr[64 * c + 2 * i]), a.scale_log2, -base));
-          const float p1 = ex2(__fmaf_rn(__uint_as_float(sr[64 * c + 2 * i + 1]), a.scale_log2, -base));
-          sum[(2 * i) & 3] += p0;
-          sum[(2 * i + 1) & 3] += p1;
-          pr[i] = pack2<T>(p0, p1);
-        }
+        if (all)
+          weights64<T, true>(sr + 64 * c, a.scale_log2, base, pr, sum);
+        else
+          weights64<T, false>(sr + 64 * c, a.scale_log2, base, pr, sum);
         tmem_st32(S_COL(t) + trow + 32 * c, pr);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tmem_wait_st();
       fence_before();
       __syncwarp();
@@ -408,7 +458,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp == PC_COPY_WARP) {
     /* ------------------------------ copies ------------------------------ */
     const int page_rows = 1 << g.page_shift, box = min(page_rows, PC_KEYS);
     constexpr int HALVES = HD / 64;

@@ -9,9 +9,10 @@
  *                   memory over S as the next product's 16-bit operand, their sum. O is multiplied in place only when a row's maximum has grown by
  *                   more than 2^7 since it was last done: until then the probabilities are that much larger, which their 16-bit type holds
  *                   (fp16: 2^8 to keep small ones out of the subnormal numbers, times 2^7).
- *   warp 8          one thread issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as it lies,
- *                   dimensions contiguous). While one tile's probabilities are computed the other tile's products run.
- *   warp 9          TMA copies of K and V tiles through one ring of slots: a box per page (128 rows of it at most) and 64 dimensions.
+ *   warps 8, 9      one for each tile; a thread issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as
+ *                   it lies, dimensions contiguous; the first 64 rows as soon as their probabilities are there). While one tile's
+ *                   probabilities are computed the other tile's products run.
+ *   warp 10         TMA copies of K and V tiles through one ring of slots: a box per page (128 rows of it at most) and 64 dimensions.
  * Tensor memory: S (P) 128 columns a tile, O head_dim columns a tile. A step's products take 4 * 128 * 128 * head_dim flop a tile, its 16384
  * exponentials as many clocks (16 a clock and SM) as its products at head_dim 128.
  * Few tiles: the CTAs of a cluster share a pair of tiles along the cache rows and join through each other's shared memory.
@@ -43,10 +44,10 @@ namespace {
 
 constexpr int PC_ROWS = 128; // of a tile: the MMA's M, lanes of tensor memory
 constexpr int PC_KEYS = 128; // cache rows of a step
-constexpr int PC_MMA_WARP = 8, PC_COPY_WARP = 9, PC_THREADS = 384; // warps 10 and 11 only make the third group of four whole
+constexpr int PC_MMA_WARP = 8, PC_COPY_WARP = 10, PC_THREADS = 384; // warp 11 only makes the third group of four whole
 /* Registers of a thread: 168 at launch (384 * 168 of the 65536); the third group gives some to the others: 2 * 208 + 88 = 3 * 168. */
 constexpr int PC_REGS_ROWS = 208, PC_REGS_REST = 88;
-constexpr float PC_LIFT = 8.f, PC_GROWTH = 7.f; // log2
+constexpr float PC_LIFT = 6.f; // log2 of what a row's greatest probability is when its maximum is taken
 constexpr uint32_t PC_POLLS = 1u << 22;
 template <int HD> struct PcCfg {
   static constexpr int TILE = 128 * HD * 2; // bytes of a tile of Q, K or V: [64 dimensions of HD][row][128 B], 128-byte swizzle
@@ -79,6 +80,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
                : "memory");
+}
+/* one lane of the warp, the same every time; as a branch that the compiler knows one lane takes */
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -125,47 +132,101 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-/* 2^x of two numbers from -126 up, x below 16, on the FMA pipes: x = n + f with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f
- * by the polynomial of the least greatest relative error with value 1 at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2),
- * n into the exponent. */
-template <typename T> __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  constexpr float MAGIC = 12582912.f;
-  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const float2 t = add2(x.x, x.y, MAGIC, MAGIC), n = add2(t.x, t.y, -MAGIC, -MAGIC), f = add2(x.x, x.y, -n.x, -n.y);
-  float2 p;
-  if constexpr (sizeof(T) == 2 && MmaType<T>::bits == 0) {
-    p = make_float2(5.590642467794357e-2f, 5.590642467794357e-2f);
-    fma2(p.x, p.y, f.x, f.y, 9.582853038422538e-3f, 9.582853038422538e-3f);
-    float2 q = make_float2(2.4024098611601802e-1f, 2.4024098611601802e-1f);
-    fma2(q.x, q.y, p.x, p.y, f.x, f.y);
-    p = make_float2(6.931241934031505e-1f, 6.931241934031505e-1f);
-    fma2(p.x, p.y, q.x, q.y, f.x, f.y);
-  } else {
-    float2 q = make_float2(2.422109594702074e-1f, 2.422109594702074e-1f);
-    fma2(q.x, q.y, f.x, f.y, 5.5008930492411165e-2f, 5.5008930492411165e-2f);
-    p = make_float2(6.932829272228233e-1f, 6.932829272228233e-1f);
-    fma2(p.x, p.y, q.x, q.y, f.x, f.y);
-  }
-  float2 r = make_float2(1.f, 1.f);
-  fma2(r.x, r.y, p.x, p.y, f.x, f.y);
-  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
-}
-
-/* 64 scores of a row to probabilities 2^(s * scale - base), packed, and their sum. ALL: none is masked; then PC_BY_FMA of every eight pairs
- * are computed beside the special function unit, which alone would take as many clocks as a step's products. */
-constexpr int PC_BY_FMA = 3;
+/* 64 scores of a row to probabilities 2^x, x = s * scale - base below 16, packed, and their sum. ALL: none is masked; then some of the pairs
+ * are computed on the FMA pipes beside the special function unit, which alone would take as many clocks as a step's products: x = n + f
+ * with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f by the polynomial of the least greatest relative error with value 1
+ * at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent. Sixteen pairs go step by step together: a warp has no
+ * other to hide the latency of its own steps. */
+constexpr int PC_BY_FMA = 6; // of sixteen pairs
 template <typename T, bool ALL>
 __device__ __forceinline__ void weights64(const uint32_t *s, float scale, float base, uint32_t *p, float2 (&sum)[2]) {
+  constexpr float MAGIC = 12582912.f;
+  constexpr int N = ALL ? PC_BY_FMA : 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    float2 x = make_float2(-base, -base);
-    fma2(x.x, x.y, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), scale, scale);
-    x = ALL && i % 8 < PC_BY_FMA ? ex2_fma<T>(x) : make_float2(ex2(x.x), ex2(x.y));
-    sum[i & 1] = add2(sum[i & 1].x, sum[i & 1].y, x.x, x.y);
-    p[i] = pack2<T>(x.x, x.y);
+  for (int g = 0; g < 2; ++g) {
+    float2 x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = make_float2(-base, -base);
+      fma2(x[i].x, x[i].y, __uint_as_float(s[32 * g + 2 * i]), __uint_as_float(s[32 * g + 2 * i + 1]), scale, scale);
+    }
+    float2 t[N + 1], f[N + 1], q[N + 1];
+    int next = N; // pairs for the special function unit, some of them after each step of the others
+    auto some = [&](int upto) {
+#pragma unroll
+      for (int i = N; i < 16; ++i)
+        if (i >= next && i < upto)
+          x[i] = make_float2(ex2(x[i].x), ex2(x[i].y));
+      next = upto;
+    };
+    if constexpr (ALL) {
+      constexpr bool FOUR = MmaType<T>::bits == 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        x[i] = make_float2(fmaxf(x[i].x, -126.f), fmaxf(x[i].y, -126.f));
+      some(N + 2);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        t[i] = add2(x[i].x, x[i].y, MAGIC, MAGIC);
+      some(N + 3);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        f[i] = add2(t[i].x, t[i].y, -MAGIC, -MAGIC);
+      some(N + 4);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        f[i] = add2(x[i].x, x[i].y, -f[i].x, -f[i].y);
+      some(N + 5);
+      if constexpr (FOUR) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          q[i] = make_float2(5.590642467794357e-2f, 5.590642467794357e-2f);
+          fma2(q[i].x, q[i].y, f[i].x, f[i].y, 9.582853038422538e-3f, 9.582853038422538e-3f);
+        }
+        some(N + 6);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        constexpr float C2 = FOUR ? 2.4024098611601802e-1f : 2.422109594702074e-1f;
+        float2 r = make_float2(C2, C2);
+        if constexpr (FOUR)
+          fma2(r.x, r.y, q[i].x, q[i].y, f[i].x, f[i].y);
+        else
+          fma2(r.x, r.y, f[i].x, f[i].y, 5.5008930492411165e-2f, 5.5008930492411165e-2f);
+        q[i] = r;
+      }
+      some(N + 7);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        constexpr float C1 = FOUR ? 6.931241934031505e-1f : 6.932829272228233e-1f;
+        float2 r = make_float2(C1, C1);
+        fma2(r.x, r.y, q[i].x, q[i].y, f[i].x, f[i].y);
+        q[i] = r;
+      }
+      some(N + 8);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float2 r = make_float2(1.f, 1.f);
+        fma2(r.x, r.y, q[i].x, q[i].y, f[i].x, f[i].y);
+        q[i] = r;
+      }
+      some(N + 10);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        x[i] = make_float2(__uint_as_float(__float_as_uint(q[i].x) + (__float_as_uint(t[i].x) << 23)),
+                           __uint_as_float(__float_as_uint(q[i].y) + (__float_as_uint(t[i].y) << 23)));
+    }
+    some(16);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      sum[i & 1] = add2(sum[i & 1].x, sum[i & 1].y, x[i].x, x[i].y);
+      p[16 * g + i] = pack2<T>(x[i].x, x[i].y);
+    }
   }
 }
+
+/* sum of a row's 128 probabilities of a step up to which each fits its 16-bit type, and m may stay */
+template <typename T> constexpr float PC_MOST = MmaType<T>::bits == 0 ? 32768.f : 1e30f;
 
 /* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. */
 __device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, int lane, int *seq, int *tile) {
@@ -201,7 +262,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t *smem = smem_raw + (sbase - smem_u32(smem_raw));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // numbers that are the same in a warp, and known to be to the compiler: the operands of MMAs are uniform registers
+  const int tid = threadIdx.x, warp = __shfl_sync(FULL, tid >> 5, 0), lane = tid & 31;
   const uint32_t bar0 = sbase + Cfg::OFF_BARS;
   // slots full and empty; Q here; of a tile: S complete, P complete, O complete
   auto FULL_BAR = [&](int i) { return bar0 + 8u * i; };
@@ -209,20 +271,22 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   const uint32_t Q_BAR = bar0 + 8 * 16;
   auto S_BAR = [&](int t) { return bar0 + 8u * (17 + t); };
   auto P_BAR = [&](int t) { return bar0 + 8u * (19 + t); };
-  auto O_BAR = [&](int t) { return bar0 + 8u * (21 + t); };
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Cfg::OFF_BARS + 192);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Cfg::OFF_BARS + 200);
+  auto O_BAR = [&](int t) { return bar0 + 8u * (23 + t); };
+  auto TURN_BAR = [&](int t) { return bar0 + 8u * (25 + t); }; // the tile's turn to issue
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Cfg::OFF_BARS + 224);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Cfg::OFF_BARS + 232);
 
   if (tid == 0) {
     for (int i = 0; i < Cfg::SLOTS; ++i) {
       mbar_init(FULL_BAR(i), 1);
-      mbar_init(EMPTY_BAR(i), 1);
+      mbar_init(EMPTY_BAR(i), 2); // both tiles
     }
     mbar_init(Q_BAR, 8);
     for (int t = 0; t < 2; ++t) {
       mbar_init(S_BAR(t), 1);
       mbar_init(P_BAR(t), 4);
       mbar_init(O_BAR(t), 1);
+      mbar_init(TURN_BAR(t), 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -234,7 +298,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(FULL, *tmem_slot, 0);
   auto S_COL = [&](int t) { return tmem + 128u * t; };
   auto O_COL = [&](int t) { return tmem + 256u + (uint32_t)HD * t; };
   pdl_launch_dependents();
@@ -277,61 +341,81 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
     float m = -INFINITY, l = 0.f; // the maximum that the row's probabilities refer to, in powers of two; their sum
     bool ok = true;
     const bool mine = t == 0 ? rows > 0 : two;
+    // The scores of step j are complete, and all products issued before them: nobody reads its keys and the values in front of them any
+    // more. (An arrival by tcgen05.commit for each slot costs the thread that issues the products time.) Where
+    // the second tile has no rows the first gives back for both.
+    auto give_back = [&](int j) {
+      if ((warp & 3) == 0 && lane == 0)
+        for (int item = max(0, 2 * j - 1); item <= 2 * j; ++item)
+          if (item + Cfg::SLOTS < 2 * steps) // nobody waits for a slot that is not filled again
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(EMPTY_BAR(item % Cfg::SLOTS)), "r"(two ? 1 : 2) : "memory");
+    };
     for (int j = 0; mine && j < steps; ++j) {
       if (!(ok = pc_wait(S_BAR(t), j & 1, abort_flag)))
         break;
+      give_back(j);
       fence_after();
-      uint32_t sr[PC_KEYS];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        tmem_ld32(S_COL(t) + trow + 32 * c, sr + 32 * c);
-      tmem_wait_ld();
       const int j0 = sight.block(b_lo + j) * PC_KEYS;
       const bool all = j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first);
-      if (!all) {
+      uint32_t pr[PC_KEYS / 2];
+      float sum;
+      // A row's probabilities refer to a maximum m that is taken in the first step, and where rows are masked. Other steps go by the m there
+      // is; what they give shows whether it does. If not the step begins again, with the maximum.
+      for (bool afresh = j == 0 || !all;; afresh = true) {
+        uint32_t sr[PC_KEYS];
 #pragma unroll
-        for (int i = 0; i < PC_KEYS; ++i) {
-          const int key = j0 + i;
-          if (!(key <= p && (key > p - a.window || key < a.first)))
-            sr[i] = 0xff800000u;
-        }
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int c = 0; c < 4; ++c)
+          tmem_ld32(S_COL(t) + trow + 32 * c, sr + 32 * c);
+        tmem_wait_ld();
+        if (afresh) {
+          if (!all) {
 #pragma unroll
-      for (int i = 0; i < PC_KEYS; i += 2)
-        mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-      const float big = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
-      const bool grown = big > m + PC_GROWTH;
-      if (__any_sync(FULL, grown)) {
-        const float keep = grown ? ex2(m - big) : 1.f;
-        l *= keep;
-        if (grown)
-          m = big;
-        if (j > 0) { // the products so far are complete: S of this step was issued behind them
+            for (int i = 0; i < PC_KEYS; ++i) {
+              const int key = j0 + i;
+              if (!(key <= p && (key > p - a.window || key < a.first)))
+                sr[i] = 0xff800000u;
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(O_COL(t) + trow + 32 * c, o);
-            tmem_wait_ld();
+          for (int i = 0; i < PC_KEYS; i += 2)
+            mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+          const float big = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
+          const bool grown = big > m;
+          if (__any_sync(FULL, grown)) {
+            const float keep = grown ? ex2(m - big) : 1.f;
+            l *= keep;
+            if (grown)
+              m = big;
+            if (j > 0) { // the products so far are complete: S of this step was issued behind them
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-            tmem_st32(O_COL(t) + trow + 32 * c, o);
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(O_COL(t) + trow + 32 * c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                tmem_st32(O_COL(t) + trow + 32 * c, o);
+              }
+            }
           }
         }
-      }
-      const float base = m == -INFINITY ? 0.f : m - PC_LIFT;
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float base = m == -INFINITY ? 0.f : m - PC_LIFT;
+        float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pr[32];
-        if (all)
-          weights64<T, true>(sr + 64 * c, a.scale_log2, base, pr, sum);
-        else
-          weights64<T, false>(sr + 64 * c, a.scale_log2, base, pr, sum);
-        tmem_st32(S_COL(t) + trow + 32 * c, pr);
+        for (int c = 0; c < 2; ++c)
+          if (all)
+            weights64<T, true>(sr + 64 * c, a.scale_log2, base, pr + 32 * c, s2);
+          else
+            weights64<T, false>(sr + 64 * c, a.scale_log2, base, pr + 32 * c, s2);
+        sum = (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y);
+        if (afresh || !__any_sync(FULL, sum > PC_MOST<T>))
+          break;
       }
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      tmem_st32(S_COL(t) + trow, pr);
+      tmem_st32(S_COL(t) + trow + 32, pr + 32);
+      l += sum;
       tmem_wait_st();
       fence_before();
       __syncwarp();
@@ -392,40 +476,42 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       if (parts > 1)
         *reinterpret_cast<float2 *>(smem + Cfg::OFF_ML + 8 * (t * PC_ROWS + row)) = make_float2(m, l);
     }
-  } else if (warp == PC_MMA_WARP) {
+  } else if (warp < PC_COPY_WARP) {
     /* ------------------------------ products ------------------------------ */
     constexpr uint32_t IDESC = 1u << 4 | MmaType<T>::bits | (uint32_t)(PC_ROWS >> 4) << 24;
     constexpr uint32_t IDESC_S = IDESC | (uint32_t)(PC_KEYS >> 3) << 17;
     constexpr uint32_t IDESC_O = IDESC | (uint32_t)(HD >> 3) << 17 | 1u << 16; // B: its rows are the K dimension
+    const int t = warp - PC_MMA_WARP;
+    const bool mine = t == 0 || two;
     auto slot_at = [&](int item) { return sbase + Cfg::OFF_RING + (item % Cfg::SLOTS) * Cfg::TILE; };
     auto here = [&](int item) { return pc_wait(FULL_BAR(item % Cfg::SLOTS), item / Cfg::SLOTS & 1, abort_flag); };
-    auto scores = [&](int t, int item) {
-      if (lane == 0) {
+    auto scores = [&](int item) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
-          mma_ss(S_COL(t), sw128_desc(sbase + t * Cfg::TILE + at, 0, 1024), sw128_desc(slot_at(item) + at, 0, 1024), IDESC_S, k != 0);
-        }
-        mma_commit(S_BAR(t));
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
+        mma_ss(S_COL(t), sw128_desc(sbase + t * Cfg::TILE + at, 0, 1024), sw128_desc(slot_at(item) + at, 0, 1024), IDESC_S, k != 0);
       }
+      mma_commit(S_BAR(t));
     };
-    auto refilled = [&](int item) { return item + Cfg::SLOTS < 2 * steps; }; // else nobody waits for the slot: no arrival may be on its way at the end
-    const int tiles = two ? 2 : 1;
-    bool ok = rows > 0 && steps > 0 && pc_wait(Q_BAR, 0, abort_flag) && here(0);
-    if (ok) {
+    // The tiles' products are issued in turn, never mixed: mixed ones are all through at the same time, and then the row threads of both tiles
+    // work while the tensor cores wait. Batch n is S of step 0, or O of step n - 1 and S of step n.
+    auto my_turn = [&](int n) { return !two || (t == 0 && n == 0) || pc_wait(TURN_BAR(t), (t == 0 ? n - 1 : n) & 1, abort_flag); };
+    auto your_turn = [&] {
+      if (two)
+        mbar_arrive(TURN_BAR(1 - t));
+    };
+    bool ok = mine && rows > 0 && steps > 0 && pc_wait(Q_BAR, 0, abort_flag) && here(0) && my_turn(0);
+    if (ok && elected()) {
       fence_after();
-      for (int t = 0; t < tiles; ++t)
-        scores(t, 0);
-      if (lane == 0 && refilled(0))
-        mma_commit(EMPTY_BAR(0));
+      scores(0);
+      your_turn();
     }
     for (int j = 0; j < steps && ok; ++j) {
-      const int vi = 2 * j + 1, ki = 2 * j + 2;
+      const int vi = 2 * j + 1, ki = 2 * j + 2, j0 = sight.block(b_lo + j) * PC_KEYS;
       if (!(ok = here(vi)))
         break;
-      const int j0 = sight.block(b_lo + j) * PC_KEYS;
       if (!(j0 + PC_KEYS - 1 <= sight.hi && (j0 >= sight.from || j0 + PC_KEYS <= sight.first))) {
-        // rows that nobody sees meet probabilities of zero: what they hold must be finite
+        // rows that nobody sees meet probabilities of zero: what they hold must be finite (both warps write the same zeros)
         for (int i = lane; i < PC_KEYS * (HD / 8); i += 32) {
           const int rr = i >> 3 & (PC_KEYS - 1);
           if (!sight.row_read(j0 + rr))
@@ -436,25 +522,19 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       }
       if (j + 1 < steps && !(ok = here(ki)))
         break;
-      for (int t = 0; t < tiles; ++t) {
-        if (!(ok = pc_wait(P_BAR(t), j & 1, abort_flag)))
-          break;
-        fence_after();
-        if (lane == 0) {
+      if (!(ok = pc_wait(P_BAR(t), j & 1, abort_flag) && my_turn(j + 1)))
+        break;
+      fence_after();
+      if (elected()) {
 #pragma unroll
-          for (int k = 0; k < PC_KEYS / 16; ++k)
-            mma_ts(O_COL(t), S_COL(t) + 8 * k, sw128_desc(slot_at(vi) + k * 2048, 128 * 128, 1024), IDESC_O, j != 0 || k != 0);
-          if (j + 1 == steps)
-            mma_commit(O_BAR(t));
-        }
-        if (j + 1 < steps)
-          scores(t, ki);
-      }
-      if (ok && lane == 0) {
-        if (refilled(vi))
-          mma_commit(EMPTY_BAR(vi % Cfg::SLOTS));
-        if (refilled(ki))
-          mma_commit(EMPTY_BAR(ki % Cfg::SLOTS));
+        for (int k = 0; k < PC_KEYS / 16; ++k)
+          mma_ts(O_COL(t), S_COL(t) + 8 * k, sw128_desc(slot_at(vi) + k * 2048, 128 * 128, 1024), IDESC_O, j != 0 || k != 0);
+        if (j + 1 == steps)
+          mma_commit(O_BAR(t));
+        else
+          scores(ki);
+        if (t == 0 || j + 1 < steps) // nobody waits for the last one
+          your_turn();
       }
     }
     __syncwarp();

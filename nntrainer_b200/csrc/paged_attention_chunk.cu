@@ -5,14 +5,14 @@
  *
  * The formulas are those of paged_attention.cu. A tile is 128 rows of (token, query head of one kv head's group); a CTA holds two of
  * them against the same cache rows, in steps of 128:
- *   warps 0-3, 4-7  a thread per row of the first / second tile: S from tensor memory, running maximum, probabilities back to tensor
+ *   warps 0-7, 8-15 two threads per row of the first / second tile, one half of the step's rows each: S from tensor memory, running maximum, probabilities back to tensor
  *                   memory over S as the next product's 16-bit operand, their sum. O is multiplied in place only when a row's maximum has grown by
  *                   more than 2^7 since it was last done: until then the probabilities are that much larger, which their 16-bit type holds
  *                   (fp16: 2^8 to keep small ones out of the subnormal numbers, times 2^7).
- *   warps 8, 9      one for each tile; a thread issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as
+ *   warps 16, 17    one for each tile; a thread issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as
  *                   it lies, dimensions contiguous; the first 64 rows as soon as their probabilities are there). While one tile's
  *                   probabilities are computed the other tile's products run.
- *   warp 10         TMA copies of K and V tiles through one ring of slots: a box per page (128 rows of it at most) and 64 dimensions.
+ *   warp 18         TMA copies of K and V tiles through one ring of slots: a box per page (128 rows of it at most) and 64 dimensions.
  * Tensor memory: S (P) 128 columns a tile, O head_dim columns a tile. A step's products take 4 * 128 * 128 * head_dim flop a tile, its 16384
  * exponentials as many clocks (16 a clock and SM) as its products at head_dim 128.
  * Few tiles: the CTAs of a cluster share a pair of tiles along the cache rows and join through each other's shared memory.
@@ -44,9 +44,11 @@ namespace {
 
 constexpr int PC_ROWS = 128; // of a tile: the MMA's M, lanes of tensor memory
 constexpr int PC_KEYS = 128; // cache rows of a step
-constexpr int PC_MMA_WARP = 8, PC_COPY_WARP = 10, PC_THREADS = 384; // warp 11 only makes the third group of four whole
-/* Registers of a thread: 168 at launch (384 * 168 of the 65536); the third group gives some to the others: 2 * 208 + 88 = 3 * 168. */
-constexpr int PC_REGS_ROWS = 208, PC_REGS_REST = 88;
+constexpr int PC_ROW_WARPS = 8; // of a tile: two threads per row, each with one half of a step's cache rows
+constexpr int PC_MMA_WARP = 2 * PC_ROW_WARPS, PC_COPY_WARP = PC_MMA_WARP + 2;
+constexpr int PC_THREADS = (PC_MMA_WARP + 4) * 32; // the last warp only makes the group of four whole
+/* Registers of a thread: 96 at launch (640 * 96 of the 65536); the last group gives some to the others: 4 * 104 + 64 = 5 * 96. */
+constexpr int PC_REGS_ROWS = 104, PC_REGS_REST = 64;
 constexpr float PC_LIFT = 6.f; // log2 of what a row's greatest probability is when its maximum is taken
 constexpr uint32_t PC_POLLS = 1u << 22;
 template <int HD> struct PcCfg {
@@ -54,7 +56,8 @@ template <int HD> struct PcCfg {
   static constexpr int SLOTS = HD == 128 ? 5 : 8;
   static constexpr int OFF_RING = 2 * TILE;
   static constexpr int OFF_BARS = OFF_RING + SLOTS * TILE;
-  static constexpr int SMEM = OFF_BARS + 256 + 1024; // the tiles begin at a multiple of 1024
+  static constexpr int OFF_PAIR = OFF_BARS + 256; // a number of each row thread for the row's other one
+  static constexpr int SMEM = OFF_PAIR + 2 * 2 * PC_ROWS * 4;
   // a CTA's part of a shared pair of tiles, in the tiles' place
   static constexpr int PITCH = HD + 4; // floats of a row: neighbours' 16-byte pieces fall into different banks
   static constexpr int OFF_ML = 2 * PC_ROWS * PITCH * 4;
@@ -107,6 +110,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
                "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
                : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+               "r"(r[14]), "r"(r[15]), "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -132,100 +147,76 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-/* 64 scores of a row to probabilities 2^x, x = s * scale - base below 16, packed, and their sum. ALL: none is masked; then some of the pairs
+/* 32 scores of a row to probabilities 2^x, x = s * scale - base below 16, packed, and their sum. ALL: none is masked; then some of the pairs
  * are computed on the FMA pipes beside the special function unit, which alone would take as many clocks as a step's products: x = n + f
  * with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f by the polynomial of the least greatest relative error with value 1
- * at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent. Sixteen pairs go step by step together: a warp has no
- * other to hide the latency of its own steps. */
-constexpr int PC_BY_FMA = 6; // of sixteen pairs
+ * at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent. */
+constexpr int PC_GROUP = 8, PC_BY_FMA = 3; // pairs that go step by step together, so many of them on the FMA pipes
 template <typename T, bool ALL>
-__device__ __forceinline__ void weights64(const uint32_t *s, float scale, float base, uint32_t *p, float2 (&sum)[2]) {
+__device__ __forceinline__ float weights32(const uint32_t *s, float scale, float base, uint32_t *p) {
   constexpr float MAGIC = 12582912.f;
+  constexpr bool FOUR = MmaType<T>::bits == 0;
   constexpr int N = ALL ? PC_BY_FMA : 0;
+  float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    float2 x[16];
+  for (int g = 0; g < 16; g += PC_GROUP) {
+    float2 x[PC_GROUP], t[PC_GROUP], f[PC_GROUP], q[PC_GROUP];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < PC_GROUP; ++i) {
       x[i] = make_float2(-base, -base);
-      fma2(x[i].x, x[i].y, __uint_as_float(s[32 * g + 2 * i]), __uint_as_float(s[32 * g + 2 * i + 1]), scale, scale);
+      fma2(x[i].x, x[i].y, __uint_as_float(s[2 * (g + i)]), __uint_as_float(s[2 * (g + i) + 1]), scale, scale);
     }
-    float2 t[N + 1], f[N + 1], q[N + 1];
-    int next = N; // pairs for the special function unit, some of them after each step of the others
-    auto some = [&](int upto) {
 #pragma unroll
-      for (int i = N; i < 16; ++i)
-        if (i >= next && i < upto)
-          x[i] = make_float2(ex2(x[i].x), ex2(x[i].y));
-      next = upto;
-    };
-    if constexpr (ALL) {
-      constexpr bool FOUR = MmaType<T>::bits == 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        x[i] = make_float2(fmaxf(x[i].x, -126.f), fmaxf(x[i].y, -126.f));
-      some(N + 2);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        t[i] = add2(x[i].x, x[i].y, MAGIC, MAGIC);
-      some(N + 3);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        f[i] = add2(t[i].x, t[i].y, -MAGIC, -MAGIC);
-      some(N + 4);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        f[i] = add2(x[i].x, x[i].y, -f[i].x, -f[i].y);
-      some(N + 5);
+    for (int i = 0; i < N; ++i) {
+      x[i] = make_float2(fmaxf(x[i].x, -126.f), fmaxf(x[i].y, -126.f));
+      t[i] = add2(x[i].x, x[i].y, MAGIC, MAGIC);
+      f[i] = add2(t[i].x, t[i].y, -MAGIC, -MAGIC);
+      f[i] = add2(x[i].x, x[i].y, -f[i].x, -f[i].y);
       if constexpr (FOUR) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          q[i] = make_float2(5.590642467794357e-2f, 5.590642467794357e-2f);
-          fma2(q[i].x, q[i].y, f[i].x, f[i].y, 9.582853038422538e-3f, 9.582853038422538e-3f);
-        }
-        some(N + 6);
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        constexpr float C2 = FOUR ? 2.4024098611601802e-1f : 2.422109594702074e-1f;
-        float2 r = make_float2(C2, C2);
-        if constexpr (FOUR)
-          fma2(r.x, r.y, q[i].x, q[i].y, f[i].x, f[i].y);
-        else
-          fma2(r.x, r.y, f[i].x, f[i].y, 5.5008930492411165e-2f, 5.5008930492411165e-2f);
-        q[i] = r;
-      }
-      some(N + 7);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        constexpr float C1 = FOUR ? 6.931241934031505e-1f : 6.932829272228233e-1f;
-        float2 r = make_float2(C1, C1);
+        q[i] = make_float2(5.590642467794357e-2f, 5.590642467794357e-2f);
+        fma2(q[i].x, q[i].y, f[i].x, f[i].y, 9.582853038422538e-3f, 9.582853038422538e-3f);
+        float2 r = make_float2(2.4024098611601802e-1f, 2.4024098611601802e-1f);
         fma2(r.x, r.y, q[i].x, q[i].y, f[i].x, f[i].y);
-        q[i] = r;
+        q[i] = make_float2(6.931241934031505e-1f, 6.931241934031505e-1f);
+        fma2(q[i].x, q[i].y, r.x, r.y, f[i].x, f[i].y);
+      } else {
+        float2 r = make_float2(2.422109594702074e-1f, 2.422109594702074e-1f);
+        fma2(r.x, r.y, f[i].x, f[i].y, 5.5008930492411165e-2f, 5.5008930492411165e-2f);
+        q[i] = make_float2(6.932829272228233e-1f, 6.932829272228233e-1f);
+        fma2(q[i].x, q[i].y, r.x, r.y, f[i].x, f[i].y);
       }
-      some(N + 8);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float2 r = make_float2(1.f, 1.f);
-        fma2(r.x, r.y, q[i].x, q[i].y, f[i].x, f[i].y);
-        q[i] = r;
-      }
-      some(N + 10);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        x[i] = make_float2(__uint_as_float(__float_as_uint(q[i].x) + (__float_as_uint(t[i].x) << 23)),
-                           __uint_as_float(__float_as_uint(q[i].y) + (__float_as_uint(t[i].y) << 23)));
+      float2 r = make_float2(1.f, 1.f);
+      fma2(r.x, r.y, q[i].x, q[i].y, f[i].x, f[i].y);
+      x[i] = make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t[i].x) << 23)),
+                         __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t[i].y) << 23)));
     }
-    some(16);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      sum[i & 1] = add2(sum[i & 1].x, sum[i & 1].y, x[i].x, x[i].y);
-      p[16 * g + i] = pack2<T>(x[i].x, x[i].y);
+    for (int i = N; i < PC_GROUP; ++i)
+      x[i] = make_float2(ex2(x[i].x), ex2(x[i].y));
+#pragma unroll
+    for (int i = 0; i < PC_GROUP; ++i) {
+      sum = add2(sum.x, sum.y, x[i].x, x[i].y);
+      p[g + i] = pack2<T>(x[i].x, x[i].y);
     }
   }
+  return sum.x + sum.y;
 }
 
-/* sum of a row's 128 probabilities of a step up to which each fits its 16-bit type, and m may stay */
+/* Barriers of a tile's row threads. They come to every one of them whatever became of their bounded waits: whether one ran out is
+ * agreed on here too, and then all leave together. */
+__device__ __forceinline__ void rows_sync(int t) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(1 + t), "n"(PC_ROW_WARPS * 32) : "memory");
+}
+__device__ __forceinline__ bool rows_any(int t, bool v) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"((uint32_t)v), "r"(1 + t), "n"(PC_ROW_WARPS * 32)
+               : "memory");
+  return r != 0;
+}
+
+/* sum of a row thread's probabilities of a step up to which each fits its 16-bit type, and m may stay */
 template <typename T> constexpr float PC_MOST = MmaType<T>::bits == 0 ? 32768.f : 1e30f;
 
 /* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. */
@@ -259,9 +250,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1)
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttendArgs a, PagedGeom g,
                              PagedBatch s) {
   using Cfg = PcCfg<HD>;
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  const uint32_t sbase = (smem_u32(smem_raw) + 1023) & ~1023u;
-  uint8_t *smem = smem_raw + (sbase - smem_u32(smem_raw));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sbase = smem_u32(smem);
   // numbers that are the same in a warp, and known to be to the compiler: the operands of MMAs are uniform registers
   const int tid = threadIdx.x, warp = __shfl_sync(FULL, tid >> 5, 0), lane = tid & 31;
   const uint32_t bar0 = sbase + Cfg::OFF_BARS;
@@ -281,10 +271,10 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       mbar_init(FULL_BAR(i), 1);
       mbar_init(EMPTY_BAR(i), 2); // both tiles
     }
-    mbar_init(Q_BAR, 8);
+    mbar_init(Q_BAR, 2 * PC_ROW_WARPS);
     for (int t = 0; t < 2; ++t) {
       mbar_init(S_BAR(t), 1);
-      mbar_init(P_BAR(t), 4);
+      mbar_init(P_BAR(t), PC_ROW_WARPS);
       mbar_init(O_BAR(t), 1);
       mbar_init(TURN_BAR(t), 1);
     }
@@ -315,18 +305,18 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   const Sight sight(r.pos + flat0 / G, any ? r.pos + (flat0 + rows - 1) / G : -1, a.window, a.first, PC_KEYS);
   const int b_lo = (int)((long long)sight.blocks * part / parts), steps = (int)((long long)sight.blocks * (part + 1) / parts) - b_lo;
 
-  if (warp >= 8)
+  if (warp >= PC_MMA_WARP)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PC_REGS_REST));
-  if (warp < 8) {
+  if (warp < PC_MMA_WARP) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PC_REGS_ROWS));
-    /* ------------------------------ a thread per row ------------------------------ */
-    const int t = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane, flat = flat0 + t * PC_ROWS + row;
+    /* ------------------------------ two threads per row ------------------------------ */
+    const int t = warp / PC_ROW_WARPS, half = warp / 4 & 1, wrow = (warp & 3) * 32, row = wrow + lane, flat = flat0 + t * PC_ROWS + row;
     const bool there = t * PC_ROWS + row < rows;
     const int p = there ? r.pos + flat / G : -1;
     constexpr int CH = HD / 8; // 16-byte pieces of a row
 #pragma unroll 4
-    for (int i = lane; i < 32 * CH; i += 32) {
-      const int rr = wrow + i / CH, c = i % CH, f = flat0 + t * PC_ROWS + rr;
+    for (int i = lane; i < 16 * CH; i += 32) {
+      const int rr = wrow + 16 * half + i / CH, c = i % CH, f = flat0 + t * PC_ROWS + rr;
       uint4 w = make_uint4(0, 0, 0, 0);
       if (t * PC_ROWS + rr < rows && 8 * c < g.hd)
         w = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (r.first + f / G) * a.ld_q + (size_t)(h * G + f % G) * g.hd + 8 * c);
@@ -338,49 +328,55 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       mbar_arrive(Q_BAR);
 
     const uint32_t trow = (uint32_t)wrow << 16;
-    float m = -INFINITY, l = 0.f; // the maximum that the row's probabilities refer to, in powers of two; their sum
+    const uint32_t s_at = S_COL(t) + trow + 64 * half, o_at = O_COL(t) + trow + HD / 2 * half; // P begins where the half's scores do
+    float *pair_own = reinterpret_cast<float *>(smem + Cfg::OFF_PAIR) + (2 * t + half) * PC_ROWS + row;
+    const float *pair_other = reinterpret_cast<const float *>(smem + Cfg::OFF_PAIR) + (2 * t + 1 - half) * PC_ROWS + row;
+    float m = -INFINITY, l = 0.f; // the maximum that the row's probabilities refer to, in powers of two; the sum of this half's
     bool ok = true;
     const bool mine = t == 0 ? rows > 0 : two;
     // The scores of step j are complete, and all products issued before them: nobody reads its keys and the values in front of them any
     // more. (An arrival by tcgen05.commit for each slot costs the thread that issues the products time.) Where
     // the second tile has no rows the first gives back for both.
     auto give_back = [&](int j) {
-      if ((warp & 3) == 0 && lane == 0)
+      if (warp % PC_ROW_WARPS == 0 && lane == 0)
         for (int item = max(0, 2 * j - 1); item <= 2 * j; ++item)
           if (item + Cfg::SLOTS < 2 * steps) // nobody waits for a slot that is not filled again
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(EMPTY_BAR(item % Cfg::SLOTS)), "r"(two ? 1 : 2) : "memory");
     };
     for (int j = 0; mine && j < steps; ++j) {
-      if (!(ok = pc_wait(S_BAR(t), j & 1, abort_flag)))
-        break;
-      give_back(j);
+      const bool came = pc_wait(S_BAR(t), j & 1, abort_flag);
       fence_after();
       const int j0 = sight.block(b_lo + j) * PC_KEYS;
       const bool all = j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first);
-      uint32_t pr[PC_KEYS / 2];
+      uint32_t pr[32];
       float sum;
       // A row's probabilities refer to a maximum m that is taken in the first step, and where rows are masked. Other steps go by the m there
       // is; what they give shows whether it does. If not the step begins again, with the maximum.
       for (bool afresh = j == 0 || !all;; afresh = true) {
-        uint32_t sr[PC_KEYS];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_ld32(S_COL(t) + trow + 32 * c, sr + 32 * c);
-        tmem_wait_ld();
-        if (afresh) {
+        auto scores = [&](int c, uint32_t(&sr)[32]) { // 32 of this half's
+          tmem_ld32(s_at + 32 * c, sr);
+          tmem_wait_ld();
           if (!all) {
 #pragma unroll
-            for (int i = 0; i < PC_KEYS; ++i) {
-              const int key = j0 + i;
+            for (int i = 0; i < 32; ++i) {
+              const int key = j0 + 64 * half + 32 * c + i;
               if (!(key <= p && (key > p - a.window || key < a.first)))
                 sr[i] = 0xff800000u;
             }
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        };
+        if (afresh) {
+          float mx[2] = {-INFINITY, -INFINITY};
+          for (int c = 0; c < 2; ++c) {
+            uint32_t sr[32];
+            scores(c, sr);
 #pragma unroll
-          for (int i = 0; i < PC_KEYS; i += 2)
-            mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-          const float big = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
+            for (int i = 0; i < 32; i += 2)
+              mx[i >> 1 & 1] = max3(mx[i >> 1 & 1], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+          }
+          *pair_own = fmaxf(mx[0], mx[1]) * a.scale_log2;
+          rows_sync(t);
+          const float big = fmaxf(*pair_own, *pair_other);
           const bool grown = big > m;
           if (__any_sync(FULL, grown)) {
             const float keep = grown ? ex2(m - big) : 1.f;
@@ -390,37 +386,42 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
             if (j > 0) { // the products so far are complete: S of this step was issued behind them
 #pragma unroll
               for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(O_COL(t) + trow + 32 * c, o);
+                uint32_t o[16];
+                tmem_ld16(o_at + 16 * c, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
+                for (int i = 0; i < 16; ++i)
                   o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                tmem_st32(O_COL(t) + trow + 32 * c, o);
+                tmem_st16(o_at + 16 * c, o);
               }
             }
           }
         }
         const float base = m == -INFINITY ? 0.f : m - PC_LIFT;
-        float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if (all)
-            weights64<T, true>(sr + 64 * c, a.scale_log2, base, pr + 32 * c, s2);
-          else
-            weights64<T, false>(sr + 64 * c, a.scale_log2, base, pr + 32 * c, s2);
-        sum = (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y);
-        if (afresh || !__any_sync(FULL, sum > PC_MOST<T>))
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sr[32];
+          scores(c, sr);
+          sum += all ? weights32<T, true>(sr, a.scale_log2, base, pr + 16 * c) : weights32<T, false>(sr, a.scale_log2, base, pr + 16 * c);
+        }
+        if (!rows_any(t, !came || (!afresh && sum > PC_MOST<T>)))
           break;
+        if (rows_any(t, !came)) {
+          ok = false;
+          break;
+        }
       }
-      tmem_st32(S_COL(t) + trow, pr);
-      tmem_st32(S_COL(t) + trow + 32, pr + 32);
+      if (!ok)
+        break;
+      tmem_st32(s_at, pr);
       l += sum;
       tmem_wait_st();
       fence_before();
       __syncwarp();
       if (lane == 0)
         mbar_arrive(P_BAR(t));
+      give_back(j); // behind what the products wait for
     }
 
     /* ------------------------------ the row's result ------------------------------ */
@@ -429,6 +430,11 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
     if (two && parts > 1 && steps > 0 && ok) // what follows is written where the other tile's products read
       ok = pc_wait(O_BAR(1 - t), 0, abort_flag);
     fence_after();
+    if (mine) {
+      *pair_own = l;
+      rows_sync(t);
+      l += *pair_other;
+    }
     if (mine && ok) {
       const int head = h * G + flat % G;
       float inv = 1.f;
@@ -441,10 +447,10 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd;
       float *part_row = reinterpret_cast<float *>(smem) + (t * PC_ROWS + row) * Cfg::PITCH;
 #pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = 0; c < HD / 64; ++c) {
         uint32_t o[32];
         if (steps > 0) {
-          tmem_ld32(O_COL(t) + trow + 32 * c, o);
+          tmem_ld32(o_at + 32 * c, o);
           tmem_wait_ld();
         } else {
 #pragma unroll
@@ -457,7 +463,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             f[k] = __uint_as_float(o[i + k]) * inv;
-          const int col = 32 * c + i;
+          const int col = HD / 2 * half + 32 * c + i;
           if (parts > 1) {
             *reinterpret_cast<float4 *>(part_row + col) = make_float4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<float4 *>(part_row + col + 4) = make_float4(f[4], f[5], f[6], f[7]);
@@ -473,7 +479,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
           }
         }
       }
-      if (parts > 1)
+      if (parts > 1 && half == 0)
         *reinterpret_cast<float2 *>(smem + Cfg::OFF_ML + 8 * (t * PC_ROWS + row)) = make_float2(m, l);
     }
   } else if (warp < PC_COPY_WARP) {
@@ -522,13 +528,13 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       }
       if (j + 1 < steps && !(ok = here(ki)))
         break;
-      if (!(ok = pc_wait(P_BAR(t), j & 1, abort_flag) && my_turn(j + 1)))
+      if (!(ok = my_turn(j + 1) && pc_wait(P_BAR(t), j & 1, abort_flag)))
         break;
       fence_after();
       if (elected()) {
 #pragma unroll
         for (int k = 0; k < PC_KEYS / 16; ++k)
-          mma_ts(O_COL(t), S_COL(t) + 8 * k, sw128_desc(slot_at(vi) + k * 2048, 128 * 128, 1024), IDESC_O, j != 0 || k != 0);
+          mma_ts(O_COL(t), S_COL(t) + 64 * (k >> 2) + 8 * (k & 3), sw128_desc(slot_at(vi) + k * 2048, 128 * 128, 1024), IDESC_O, j != 0 || k != 0);
         if (j + 1 == steps)
           mma_commit(O_BAR(t));
         else
@@ -578,8 +584,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   if (parts > 1) {
     cluster_sync();
     const uint32_t raised = neighbour_raised(smem_u32(const_cast<int *>(abort_flag)), lane);
-    if (warp < 8 && !__any_sync(FULL, raised)) {
-      for (int R = part + parts * warp; R < rows; R += parts * 8) {
+    if (warp < PC_MMA_WARP && !__any_sync(FULL, raised)) {
+      for (int R = part + parts * warp; R < rows; R += parts * PC_MMA_WARP) {
         const int flat = flat0 + R, head = h * G + flat % G, col = 4 * lane;
         float2 ml[8];
         float4 v[8];

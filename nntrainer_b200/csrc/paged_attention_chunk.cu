@@ -219,12 +219,28 @@ __device__ __forceinline__ bool rows_any(int t, bool v) {
 /* sum of a row thread's probabilities of a step up to which each fits its 16-bit type, and m may stay */
 template <typename T> constexpr float PC_MOST = MmaType<T>::bits == 0 ? 32768.f : 1e30f;
 
-/* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. */
+/* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. What takes
+ * longest comes first, so that it does not begin when the rest is done: in a sequence the last queries, which see most, and among up to
+ * 32 sequences those with the longest context. */
 __device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, int lane, int *seq, int *tile) {
+  auto pairs_of = [&](int b) { return b < s.batch ? (seq_rows(s, b).n * G + 2 * PC_ROWS - 1) / (2 * PC_ROWS) : 0; };
+  if (s.batch <= 32) {
+    const int n = pairs_of(lane), rows = lane < s.batch ? __ldg(s.context + lane) : 0;
+    int in_front = 0;
+    for (int b = 0; b < s.batch; ++b) {
+      const int nb = __shfl_sync(FULL, n, b), rb = __shfl_sync(FULL, rows, b);
+      in_front += rb > rows || (rb == rows && b < lane) ? nb : 0;
+    }
+    const unsigned m = __ballot_sync(FULL, work >= in_front && work < in_front + n);
+    if (!m)
+      return false;
+    *seq = __ffs(m) - 1;
+    *tile = __shfl_sync(FULL, in_front + n - 1 - work, *seq);
+    return true;
+  }
   int before = 0;
   for (int b0 = 0; b0 < s.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const int n = b < s.batch ? (seq_rows(s, b).n * G + 2 * PC_ROWS - 1) / (2 * PC_ROWS) : 0;
+    const int n = pairs_of(b0 + lane);
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -235,7 +251,7 @@ __device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, 
     if (m) {
       const int l = __ffs(m) - 1;
       *seq = b0 + l;
-      *tile = work - before - __shfl_sync(FULL, upto - n, l);
+      *tile = __shfl_sync(FULL, before + upto - 1 - work, l);
       return true;
     }
     before += __shfl_sync(FULL, upto, 31);
@@ -294,9 +310,9 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   pdl_launch_dependents();
   pdl_wait();
 
-  const int parts = cluster_size(), part = cluster_rank(), G = g.hq / g.hkv, h = blockIdx.y;
+  const int parts = cluster_size(), part = cluster_rank(), G = g.hq / g.hkv, item = blockIdx.x / parts, h = item % g.hkv;
   int seq = 0, tile = 0;
-  const bool any = find_pair(s, G, blockIdx.x / parts, lane, &seq, &tile); // the same in every CTA of a cluster
+  const bool any = find_pair(s, G, item / g.hkv, lane, &seq, &tile); // the same in every CTA of a cluster
   SeqRows r = {};
   if (any)
     r = seq_rows(s, seq);
@@ -573,7 +589,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         tma_box4(sbase + Cfg::OFF_RING + slot * Cfg::TILE + half * (PC_KEYS * 128) + at_row * 128, i & 1 ? &vmap : &kmap, half * 64, row, h, page,
                  FULL_BAR(slot));
     }
-    if (blockIdx.x == 0 && blockIdx.y == 0) // one that has no rows has no CTA either
+    if (blockIdx.x == 0) // one that has no rows has no CTA either
       for (int b = lane; b < s.batch; b += 32)
         if (seq_rows(s, b).bad)
           atomicExch(&g_paged_chunk_status, NNTR_CUDA_ERR_INVALID);
@@ -660,9 +676,23 @@ static int launch_chunk(const AttendArgs &a, const PagedGeom &g, const PagedBatc
   const long long pairs = std::min(s.batch * (((long long)s.max_new * G + pair - 1) / pair), (long long)s.tokens * G / pair + s.batch);
   const long long seen = std::min<long long>((long long)a.window + a.first + s.max_new, max_rows ? max_rows : s.table_rows);
   const long long blocks = (seen + PC_KEYS - 1) / PC_KEYS;
+  // In how many parts a pair of tiles is cut, by the steps that the last CTA ends after: waves of as many clusters as run at a time, each
+  // of a part's steps and about three more for its start; joining the parts takes about as long as two. (2 x 2048 tokens at up to
+  // 16384 rows: 512 pairs on 148 SMs are 4 waves of 120 steps, in two parts 7 of 60.)
+  static ClusterFit fit;
+  const long long items = pairs * g.hkv;
   int parts = 1;
-  while (parts < 8 && 2 * pairs * g.hkv * parts <= sm_count() && blocks >= 4 * parts)
-    parts *= 2;
+  long long least = 0;
+  for (int p = 1; p <= 8 && blocks >= 2 * p; p *= 2) {
+    const int at_once = p == 1 ? sm_count() : fit(kernel, p, PC_THREADS, smem);
+    if (at_once <= 0)
+      break;
+    const long long steps = (items + at_once - 1) / at_once * ((blocks + p - 1) / p + (p > 1 ? 5 : 3));
+    if (p == 1 || steps < least) {
+      least = steps;
+      parts = p;
+    }
+  }
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.attrs = attr;
@@ -677,7 +707,9 @@ static int launch_chunk(const AttendArgs &a, const PagedGeom &g, const PagedBatc
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  cfg.gridDim = dim3((unsigned)(pairs * parts), (unsigned)g.hkv);
+  if (items * parts > 0x7fffffffll)
+    return set_error(NNTR_CUDA_ERR_UNSUPPORTED, "paged_attention: too many rows in one call");
+  cfg.gridDim = dim3((unsigned)(items * parts));
   cfg.blockDim = dim3(PC_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;

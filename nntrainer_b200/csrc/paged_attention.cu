@@ -16,6 +16,7 @@
 #include "pipeline.cuh"
 
 #include <algorithm>
+#include <climits>
 
 namespace nntr {
 
@@ -82,9 +83,29 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int parts = cluster_size(), part = cluster_rank();
-  const int tile = blockIdx.x / parts, h = blockIdx.y, seq = blockIdx.z;
+  const int tile = blockIdx.x / parts, h = blockIdx.y;
   pdl_launch_dependents();
   pdl_wait();
+  // Long contexts begin first: of up to 128 sequences (one per thread) the one with as many longer ones as CTAs are in front
+  int seq = blockIdx.z;
+  if (s.batch > 1 && s.batch <= PD_WARPS * 32) {
+    int *rows_of = reinterpret_cast<int *>(smem), *chosen = rows_of + PD_WARPS * 32;
+    const int b = threadIdx.x, mine = b < s.batch ? __ldg(s.context + b) : 0;
+    rows_of[b] = b < s.batch ? mine : INT_MIN;
+    __syncthreads();
+    int longer = 0;
+#pragma unroll 4
+    for (int i = 0; i < s.batch; i += 4) {
+      const int4 v = *reinterpret_cast<const int4 *>(rows_of + i);
+      longer += (v.x > mine || (v.x == mine && i < b)) + (v.y > mine || (v.y == mine && i + 1 < b)) + (v.z > mine || (v.z == mine && i + 2 < b)) +
+                (v.w > mine || (v.w == mine && i + 3 < b));
+    }
+    if (b < s.batch && longer == (int)blockIdx.z)
+      *chosen = b;
+    __syncthreads();
+    seq = *chosen;
+    __syncthreads(); // the ring begins here
+  }
   const SeqRows r = seq_rows(s, seq);
   if (r.bad && threadIdx.x == 0)
     atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
@@ -307,12 +328,29 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
 /* ------------------------------------------------------------------ launch */
 
 template <typename T, int HD>
-static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch &s, int parts, int tiles, unsigned flags, cudaStream_t st) {
+static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch &s, unsigned max_rows, int tiles, unsigned flags, cudaStream_t st) {
   auto kernel = paged_attention_few_kernel<T, HD>;
   constexpr int smem = PdCfg<HD>::SMEM;
   static SmemOptIn opt_in;
   if (const int rc = opt_in(kernel, smem))
     return rc;
+  // In how many parts a sequence's rows are cut: as for chunks (paged_attention_chunk.cu), in blocks of a CTA
+  static ClusterFit fit;
+  const long long items = (long long)tiles * g.hkv * s.batch;
+  const long long seen = std::min<long long>((long long)a.window + a.first + s.max_new, max_rows ? max_rows : s.table_rows);
+  const long long blocks = (seen + PD_KEYS - 1) / PD_KEYS;
+  int parts = 1;
+  long long least = 0;
+  for (int p = 1; p <= 8 && blocks >= 2 * PD_WARPS * p; p *= 2) {
+    const int at_once = p == 1 ? 2 * sm_count() : fit(kernel, p, PD_WARPS * 32, smem);
+    if (at_once <= 0)
+      break;
+    const long long time = (items + at_once - 1) / at_once * ((blocks + p - 1) / p + (p > 1 ? 12 : 8));
+    if (p == 1 || time < least) {
+      least = time;
+      parts = p;
+    }
+  }
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.attrs = attr;
@@ -363,16 +401,10 @@ int launch_paged_attention(const nntr_paged_cache *c, const nntr_paged_batch *b,
   if (s.max_new * (g.hq / g.hkv) > 16)
     return launch_paged_attention_chunk(a, c->dtype, g, s, b->max_rows, flags, st);
   const int G = g.hq / g.hkv, tiles = (int)(((long long)s.max_new * G + 15) / 16);
-  const long long items = (long long)tiles * g.hkv * s.batch;
-  long long seen = std::min<long long>((long long)a.window + a.first + s.max_new, b->max_rows ? b->max_rows : NONE);
-  const long long blocks = (seen + PD_KEYS - 1) / PD_KEYS;
-  int parts = 1;
-  while (parts < 8 && items * parts < 2 * sm_count() && blocks >= 2ll * 2 * parts * PD_WARPS)
-    parts *= 2;
   if (c->dtype == NNTR_F16)
-    return g.hd <= 64 ? launch_few<__half, 64>(a, g, s, parts, tiles, flags, st) : launch_few<__half, 128>(a, g, s, parts, tiles, flags, st);
-  return g.hd <= 64 ? launch_few<__nv_bfloat16, 64>(a, g, s, parts, tiles, flags, st)
-                    : launch_few<__nv_bfloat16, 128>(a, g, s, parts, tiles, flags, st);
+    return g.hd <= 64 ? launch_few<__half, 64>(a, g, s, b->max_rows, tiles, flags, st) : launch_few<__half, 128>(a, g, s, b->max_rows, tiles, flags, st);
+  return g.hd <= 64 ? launch_few<__nv_bfloat16, 64>(a, g, s, b->max_rows, tiles, flags, st)
+                    : launch_few<__nv_bfloat16, 128>(a, g, s, b->max_rows, tiles, flags, st);
 }
 
 } // namespace nntr

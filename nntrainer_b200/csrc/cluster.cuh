@@ -94,31 +94,33 @@ cudaError_t launch_in_clusters(void (*kernel)(P...), dim3 grid, int parts, int t
   return cudaLaunchKernelEx(&cfg, kernel, (P)args...);
 }
 
-/** Lets a kernel have more dynamic shared memory than the default, per device, once. */
+/** Lets a kernel have more dynamic shared memory than the default, per device, once; big: and clusters of 16 CTAs. */
 struct SmemOptIn {
   std::atomic<bool> done[64];
 
-  template <typename... P> int operator()(void (*kernel)(P...), int smem) {
+  template <typename... P> int operator()(void (*kernel)(P...), int smem, bool big = false) {
     int dev = 0;
     NNTR_CHECK_CUDA(cudaGetDevice(&dev));
     if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire))
       return NNTR_CUDA_OK;
     NNTR_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (big)
+      NNTR_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (dev >= 0 && dev < 64)
       done[dev].store(true, std::memory_order_release);
     return NNTR_CUDA_OK;
   }
 };
 
-/** Clusters of 2, 4 or 8 CTAs of one kernel that run at the same time, per device, asked for once. */
+/** Clusters of 2, 4, 8 or 16 CTAs of one kernel that run at the same time, per device, asked for once. */
 struct ClusterFit {
-  std::atomic<int> n[64][3];
+  std::atomic<int> n[64][4];
 
   template <typename... P> int operator()(void (*kernel)(P...), int parts, int threads, int smem) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64)
       return 0;
-    std::atomic<int> &slot = n[dev][parts == 2 ? 0 : parts == 4 ? 1 : 2];
+    std::atomic<int> &slot = n[dev][parts == 2 ? 0 : parts == 4 ? 1 : parts == 8 ? 2 : 3];
     int v = slot.load(std::memory_order_relaxed);
     if (v == 0) {
       cudaLaunchAttribute attr[1];

@@ -138,6 +138,11 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
   auto my_block = [&](int i) { return sight.block((i * parts + part) * PD_WARPS + warp); };
   // a lane keeps the address of one of the next 32 blocks, so that the way over the page table is taken once for all of them
   long long at = 0;
+  constexpr int CHUNKS = HD / 8, STEP = 32 / CHUNKS; // 16-byte pieces of a row; rows that the lanes take at a time
+  const int c0 = lane % CHUNKS, r0 = lane / CHUNKS;
+  const long long pitch = (long long)g.hkv * g.hd, lane_at = r0 * pitch + 8 * c0;
+  // rows' pieces are spread over the banks for ldmatrix: piece c of a row lies at c ^ (row & 7)
+  const uint32_t lane_to = ring + r0 * (HD * 2) + ((c0 ^ r0) << 4);
   auto fetch = [&](int i) {
     if (i < n_mine) {
       if (i % 32 == 0)
@@ -146,16 +151,21 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
       const int j0 = my_block(i) * PD_KEYS;
       if (off < 0 && lane == 0)
         atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
-      constexpr int CHUNKS = HD / 8; // of a row
-      const uint32_t dst = ring + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES;
+      const uint32_t dst = lane_to + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES;
+      const bool whole = off >= 0 && j0 + PD_KEYS - 1 <= sight.hi && (j0 >= sight.from || j0 + PD_KEYS <= sight.first) && 8 * c0 < g.hd;
+      const T *kp = static_cast<const T *>(a.k) + (off < 0 ? 0 : off + lane_at), *vp = static_cast<const T *>(a.v) + (off < 0 ? 0 : off + lane_at);
 #pragma unroll
-      for (int u = 0; u < PD_KEYS * CHUNKS / 32; ++u) {
-        const int c = lane % CHUNKS, row = lane / CHUNKS + u * (32 / CHUNKS);
-        const bool there = off >= 0 && sight.row_read(j0 + row) && 8 * c < g.hd;
-        const long long e = there ? off + (long long)row * g.hkv * g.hd + 8 * c : 0;
-        const uint32_t to = dst + row * (HD * 2) + ((c ^ (row & 7)) << 4); // rows' pieces spread over the banks for ldmatrix
-        cp16(to, static_cast<const T *>(a.k) + e, there ? 16 : 0);
-        cp16(to + Cfg::KV_BYTES, static_cast<const T *>(a.v) + e, there ? 16 : 0);
+      for (int u = 0; u < PD_KEYS / STEP; ++u) {
+        const uint32_t to = (dst + u * STEP * (HD * 2)) ^ ((u * STEP & 7) << 4);
+        int bytes = 16;
+        if (!whole) {
+          const bool there = off >= 0 && sight.row_read(j0 + r0 + u * STEP) && 8 * c0 < g.hd;
+          bytes = there ? 16 : 0;
+        }
+        cp16(to, bytes ? kp : static_cast<const T *>(a.k), bytes);
+        cp16(to + Cfg::KV_BYTES, bytes ? vp : static_cast<const T *>(a.v), bytes);
+        kp += STEP * pitch;
+        vp += STEP * pitch;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -174,15 +184,15 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
     __syncwarp();
     const uint32_t kt = ring + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES, vt = kt + Cfg::KV_BYTES;
     const int j0 = my_block(i) * PD_KEYS;
-    float sc[2][4] = {};
+    float sc[2][4] = {}, odd[2][4] = {}; // two sums each: shorter chains
     { // four 8 x 8 matrices: keys 0-7 and 8-15, each with the lower and the upper 8 of 16 dimensions
       const int row = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
       for (int c = 0; c < HD / 16; ++c) {
         uint32_t b[4];
         ldsm4(b, kt + row * (HD * 2) + (((2 * c + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
-        mma16816<T>(sc[0], qf[c], b[0], b[1]);
-        mma16816<T>(sc[1], qf[c], b[2], b[3]);
+        mma16816<T>(c & 1 ? odd[0] : sc[0], qf[c], b[0], b[1]);
+        mma16816<T>(c & 1 ? odd[1] : sc[1], qf[c], b[2], b[3]);
       }
     }
     const bool whole = j0 + PD_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PD_KEYS <= a.first);
@@ -191,7 +201,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = j0 + 8 * t + 2 * gc + (e & 1), p = row_pos[e >> 1];
-        sc[t][e] = whole || (j <= p && (j > p - a.window || j < a.first)) ? sc[t][e] * a.scale_log2 : -INFINITY;
+        sc[t][e] = whole || (j <= p && (j > p - a.window || j < a.first)) ? (sc[t][e] + odd[t][e]) * a.scale_log2 : -INFINITY;
       }
     uint32_t pf[4];
 #pragma unroll
@@ -332,7 +342,7 @@ static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch 
   auto kernel = paged_attention_few_kernel<T, HD>;
   constexpr int smem = PdCfg<HD>::SMEM;
   static SmemOptIn opt_in;
-  if (const int rc = opt_in(kernel, smem))
+  if (const int rc = opt_in(kernel, smem, true))
     return rc;
   // In how many parts a sequence's rows are cut: as for chunks (paged_attention_chunk.cu), in blocks of a CTA
   static ClusterFit fit;
@@ -341,7 +351,7 @@ static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch 
   const long long blocks = (seen + PD_KEYS - 1) / PD_KEYS;
   int parts = 1;
   long long least = 0;
-  for (int p = 1; p <= 8 && blocks >= 2 * PD_WARPS * p; p *= 2) {
+  for (int p = 1; p <= 16 && blocks >= 2 * PD_WARPS * p; p *= 2) {
     const int at_once = p == 1 ? 2 * sm_count() : fit(kernel, p, PD_WARPS * 32, smem);
     if (at_once <= 0)
       break;

@@ -40,14 +40,13 @@ int read_paged_attn_status(int *out, bool clear) {
  * block i, probabilities straight from the accumulators to the operand of the second product. The warps of a CTA join through
  * shared memory, the CTAs of a cluster, which share the cache rows of one (sequence, kv head, tile), through each other's.
  * Bandwidth bounds it: 2 * 2 * head_dim bytes per cache row and kv head. */
-constexpr int PD_WARPS = 4;
 constexpr int PD_KEYS = 16; // of a block: no more than the smallest page
-template <int HD> struct PdCfg {
+template <int HD, int W> struct PdCfg { // W warps
   static constexpr int STAGES = HD == 128 ? 3 : 6;
   static constexpr int KV_BYTES = PD_KEYS * HD * 2;
   static constexpr int RING = STAGES * 2 * KV_BYTES;              // of a warp
   static constexpr int PART = (16 * HD + 32) * 4;                 // O, m, l of a warp or a CTA
-  static constexpr int SMEM = PD_WARPS * (RING > PART ? RING : PART) + PART;
+  static constexpr int SMEM = W * (RING > PART ? RING : PART) + PART;
 };
 
 template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -77,9 +76,9 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-template <typename T, int HD>
-__global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(AttendArgs a, PagedGeom g, PagedBatch s) {
-  using Cfg = PdCfg<HD>;
+template <typename T, int HD, int W>
+__global__ void __launch_bounds__(W * 32) paged_attention_few_kernel(AttendArgs a, PagedGeom g, PagedBatch s) {
+  using Cfg = PdCfg<HD, W>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int parts = cluster_size(), part = cluster_rank();
@@ -88,8 +87,8 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
   pdl_wait();
   // Long contexts begin first: of up to 128 sequences (one per thread) the one with as many longer ones as CTAs are in front
   int seq = blockIdx.z;
-  if (s.batch > 1 && s.batch <= PD_WARPS * 32) {
-    int *rows_of = reinterpret_cast<int *>(smem), *chosen = rows_of + PD_WARPS * 32;
+  if (s.batch > 1 && s.batch <= W * 32) {
+    int *rows_of = reinterpret_cast<int *>(smem), *chosen = rows_of + W * 32;
     const int b = threadIdx.x, mine = b < s.batch ? __ldg(s.context + b) : 0;
     rows_of[b] = b < s.batch ? mine : INT_MIN;
     __syncthreads();
@@ -134,8 +133,8 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
   }
 
   const uint32_t ring = smem_u32(smem) + warp * Cfg::RING;
-  const int n_mine = sight.blocks > part * PD_WARPS + warp ? (sight.blocks - part * PD_WARPS - warp + parts * PD_WARPS - 1) / (parts * PD_WARPS) : 0;
-  auto my_block = [&](int i) { return sight.block((i * parts + part) * PD_WARPS + warp); };
+  const int n_mine = sight.blocks > part * W + warp ? (sight.blocks - part * W - warp + parts * W - 1) / (parts * W) : 0;
+  auto my_block = [&](int i) { return sight.block((i * parts + part) * W + warp); };
   // a lane keeps the address of one of the next 32 blocks, so that the way over the page table is taken once for all of them
   long long at = 0;
   constexpr int CHUNKS = HD / 8, STEP = 32 / CHUNKS; // 16-byte pieces of a row; rows that the lanes take at a time
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
     *total = lsum;
     return sum;
   };
-  constexpr int OWN = PD_WARPS * (Cfg::RING > Cfg::PART ? Cfg::RING : Cfg::PART); // bytes in front of the CTA's part
+  constexpr int OWN = W * (Cfg::RING > Cfg::PART ? Cfg::RING : Cfg::PART); // bytes in front of the CTA's part
   float *cta = reinterpret_cast<float *>(smem + OWN);
   auto of_warp = [&](int i, int e, int n) {
     const float *p = reinterpret_cast<const float *>(smem) + i * (Cfg::PART / 4) + e;
@@ -305,12 +304,12 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
     else
       *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + e) = make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
   };
-  for (int i = threadIdx.x; i < 16 * HD / 4; i += PD_WARPS * 32) {
+  for (int i = threadIdx.x; i < 16 * HD / 4; i += W * 32) {
     const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
     if (row >= rows || col >= g.hd)
       continue;
     float mx, total;
-    const float4 sum = joined(PD_WARPS, of_warp, row, col, &mx, &total);
+    const float4 sum = joined(W, of_warp, row, col, &mx, &total);
     if (parts == 1) {
       store(row, col, sum, mx, total);
       continue;
@@ -324,7 +323,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
   if (parts == 1)
     return;
   cluster_sync();
-  for (int i = part * PD_WARPS * 32 + threadIdx.x; i < 16 * HD / 4; i += parts * PD_WARPS * 32) {
+  for (int i = part * W * 32 + threadIdx.x; i < 16 * HD / 4; i += parts * W * 32) {
     const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
     if (row >= rows || col >= g.hd)
       continue;
@@ -337,10 +336,10 @@ __global__ void __launch_bounds__(PD_WARPS * 32) paged_attention_few_kernel(Atte
 
 /* ------------------------------------------------------------------ launch */
 
-template <typename T, int HD>
+template <typename T, int HD, int W>
 static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch &s, unsigned max_rows, int tiles, unsigned flags, cudaStream_t st) {
-  auto kernel = paged_attention_few_kernel<T, HD>;
-  constexpr int smem = PdCfg<HD>::SMEM;
+  auto kernel = paged_attention_few_kernel<T, HD, W>;
+  constexpr int smem = PdCfg<HD, W>::SMEM;
   static SmemOptIn opt_in;
   if (const int rc = opt_in(kernel, smem, true))
     return rc;
@@ -351,8 +350,8 @@ static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch 
   const long long blocks = (seen + PD_KEYS - 1) / PD_KEYS;
   int parts = 1;
   long long least = 0;
-  for (int p = 1; p <= 16 && blocks >= 2 * PD_WARPS * p; p *= 2) {
-    const int at_once = p == 1 ? 2 * sm_count() : fit(kernel, p, PD_WARPS * 32, smem);
+  for (int p = 1; p <= 16 && blocks >= 2 * W * p; p *= 2) {
+    const int at_once = p == 1 ? (W == 4 ? 2 : 1) * sm_count() : fit(kernel, p, W * 32, smem);
     if (at_once <= 0)
       break;
     const long long time = (items + at_once - 1) / at_once * ((blocks + p - 1) / p + (p > 1 ? 12 : 8));
@@ -361,6 +360,10 @@ static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch 
       parts = p;
     }
   }
+  // No more CTAs than SMs: one with more warps has more rows on their way. (One stream of 32768 rows, 8 kv heads of 128: 52 us with four warps.)
+  if constexpr (W == 4)
+    if (items * parts <= sm_count() && blocks >= 4ll * W * parts)
+      return launch_few<T, HD, 8>(a, g, s, max_rows, tiles, flags, st);
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.attrs = attr;
@@ -377,7 +380,7 @@ static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch 
     ++cfg.numAttrs;
   }
   cfg.gridDim = dim3((unsigned)(tiles * parts), (unsigned)g.hkv, (unsigned)s.batch);
-  cfg.blockDim = dim3(PD_WARPS * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, g, s);
@@ -412,9 +415,9 @@ int launch_paged_attention(const nntr_paged_cache *c, const nntr_paged_batch *b,
     return launch_paged_attention_chunk(a, c->dtype, g, s, b->max_rows, flags, st);
   const int G = g.hq / g.hkv, tiles = (int)(((long long)s.max_new * G + 15) / 16);
   if (c->dtype == NNTR_F16)
-    return g.hd <= 64 ? launch_few<__half, 64>(a, g, s, b->max_rows, tiles, flags, st) : launch_few<__half, 128>(a, g, s, b->max_rows, tiles, flags, st);
-  return g.hd <= 64 ? launch_few<__nv_bfloat16, 64>(a, g, s, b->max_rows, tiles, flags, st)
-                    : launch_few<__nv_bfloat16, 128>(a, g, s, b->max_rows, tiles, flags, st);
+    return g.hd <= 64 ? launch_few<__half, 64, 4>(a, g, s, b->max_rows, tiles, flags, st) : launch_few<__half, 128, 4>(a, g, s, b->max_rows, tiles, flags, st);
+  return g.hd <= 64 ? launch_few<__nv_bfloat16, 64, 4>(a, g, s, b->max_rows, tiles, flags, st)
+                    : launch_few<__nv_bfloat16, 128, 4>(a, g, s, b->max_rows, tiles, flags, st);
 }
 
 } // namespace nntr

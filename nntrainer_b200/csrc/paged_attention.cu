@@ -8,15 +8,17 @@
  *   out = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m)), m = max_j s_j; zeros where nothing is seen
  *
  * Scores, maxima, sums and results are fp32. The probabilities are rounded to the cache's 16-bit type, the operand type of the
- * tensor cores (2^-11 or 2^-8 of each, which the sum over the rows averages out); fp16 ones are kept 2^10 times as large, so
- * that the small ones of a long context stay out of its subnormal numbers.
+ * tensor cores (2^-11 or 2^-8 of each, which the sum over the rows averages out); the greatest is kept near 2^6, so
+ * that the small ones of a long context stay out of the subnormal numbers of fp16.
  */
 #include "cluster.cuh"
 #include "paged_attention.cuh"
 #include "pipeline.cuh"
+#include "tma_map.cuh"
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace nntr {
 
@@ -36,17 +38,22 @@ int read_paged_attn_status(int *out, bool clear) {
 /* ------------------------------------------------------ a few query rows */
 
 /* Rows of a tile are (token, query head of the kv head's group), 16 of them: one M of the warp MMA. Every warp takes blocks of 16
- * cache rows in turn through a ring of its own, so that nothing but the end is shared: cp.async for block i + stages, scores of
- * block i, probabilities straight from the accumulators to the operand of the second product. The warps of a CTA join through
- * shared memory, the CTAs of a cluster, which share the cache rows of one (sequence, kv head, tile), through each other's.
- * Bandwidth bounds it: 2 * 2 * head_dim bytes per cache row and kv head. */
+ * cache rows in turn through a ring of its own, which one lane fills by TMA (a box of 16 rows and 64 dimensions), so that nothing but the
+ * end is shared: scores of the block, probabilities straight from the accumulators to the operand of the second product. The
+ * warps of a CTA join through shared memory, the CTAs of a cluster, which share the cache rows of one (sequence, kv head, tile),
+ * through each other's.
+ * Bandwidth bounds it: 2 * 2 * head_dim bytes per cache row and kv head. 64 streams of 150 to 8192 rows, 8 kv heads of 128: 172 us, 6444
+ * GB/s. */
 constexpr int PD_KEYS = 16; // of a block: no more than the smallest page
+constexpr uint32_t PD_POLLS = 1u << 22;
 template <int HD, int W> struct PdCfg { // W warps
   static constexpr int STAGES = HD == 128 ? 3 : 6;
-  static constexpr int KV_BYTES = PD_KEYS * HD * 2;
-  static constexpr int RING = STAGES * 2 * KV_BYTES;              // of a warp
-  static constexpr int PART = (16 * HD + 32) * 4;                 // O, m, l of a warp or a CTA
-  static constexpr int SMEM = W * (RING > PART ? RING : PART) + PART;
+  static constexpr int KV_BYTES = PD_KEYS * HD * 2; // [64 dimensions of HD][row][128 B], 128-byte swizzle
+  static constexpr int RING = STAGES * 2 * KV_BYTES; // of a warp
+  static constexpr int PART = (16 * HD + 32) * 4;    // O and (m, l) of a warp or a CTA
+  static_assert(RING >= PART && RING % 1024 == 0, "the warps' parts lie in the rings' place");
+  static constexpr int OFF_PART = W * RING, OFF_BARS = OFF_PART + PART;
+  static constexpr int SMEM = OFF_BARS + W * STAGES * 8 + 16;
 };
 
 template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -72,25 +79,67 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-/* 16 bytes to shared memory, zeros where `bytes` is 0 (nothing is read then) */
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
+
+/* Parts of a row's result, four of O's columns, joined one after the other, up to four on their way at a time: load(i, &v, &ml). */
+struct Joined {
+  float4 sum;
+  float m, l;
+
+  template <class Load> __device__ __forceinline__ Joined(int n, Load load) : sum(make_float4(0.f, 0.f, 0.f, 0.f)), m(-INFINITY), l(0.f) {
+    for (int i0 = 0; i0 < n; i0 += 4) {
+      float4 v[4];
+      float2 ml[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        load(min(i0 + k, n - 1), &v[k], &ml[k]);
+      float big = m;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        big = fmaxf(big, ml[k].x);
+      if (big == -INFINITY)
+        continue;
+      const float keep = ex2(m - big);
+      sum = make_float4(sum.x * keep, sum.y * keep, sum.z * keep, sum.w * keep);
+      l *= keep;
+      m = big;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i0 + k < n) {
+          const float w = ex2(ml[k].x - big);
+          sum = make_float4(sum.x + w * v[k].x, sum.y + w * v[k].y, sum.z + w * v[k].z, sum.w + w * v[k].w);
+          l += w * ml[k].y;
+        }
+    }
+  }
+};
+
 template <typename T, int HD, int W>
-__global__ void __launch_bounds__(W * 32) paged_attention_few_kernel(AttendArgs a, PagedGeom g, PagedBatch s) {
+__global__ void __launch_bounds__(W * 32)
+paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttendArgs a, PagedGeom g,
+                           PagedBatch s) {
   using Cfg = PdCfg<HD, W>;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int parts = cluster_size(), part = cluster_rank();
   const int tile = blockIdx.x / parts, h = blockIdx.y;
+  const uint32_t bars = smem_u32(smem) + Cfg::OFF_BARS + warp * Cfg::STAGES * 8;
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Cfg::OFF_BARS + W * Cfg::STAGES * 8);
   pdl_launch_dependents();
+  if (lane == 0) {
+    for (int i = 0; i < Cfg::STAGES; ++i)
+      mbar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0)
+    *abort_flag = 0;
   pdl_wait();
   // Long contexts begin first: of up to 128 sequences (one per thread) the one with as many longer ones as CTAs are in front
   int seq = blockIdx.z;
-  if (s.batch > 1 && s.batch <= W * 32) {
-    int *rows_of = reinterpret_cast<int *>(smem), *chosen = rows_of + W * 32;
+  if (s.batch > 1 && s.batch <= 128) {
+    int *rows_of = reinterpret_cast<int *>(smem), *chosen = rows_of + 128;
     const int b = threadIdx.x, mine = b < s.batch ? __ldg(s.context + b) : 0;
-    rows_of[b] = b < s.batch ? mine : INT_MIN;
+    if (b < 128)
+      rows_of[b] = b < s.batch ? mine : INT_MIN;
     __syncthreads();
     int longer = 0;
 #pragma unroll 4
@@ -103,8 +152,9 @@ __global__ void __launch_bounds__(W * 32) paged_attention_few_kernel(AttendArgs 
       *chosen = b;
     __syncthreads();
     seq = *chosen;
-    __syncthreads(); // the ring begins here
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the rings begin here
   }
+  __syncthreads();
   const SeqRows r = seq_rows(s, seq);
   if (r.bad && threadIdx.x == 0)
     atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
@@ -113,6 +163,35 @@ __global__ void __launch_bounds__(W * 32) paged_attention_few_kernel(AttendArgs 
     return; // every CTA of the cluster alike
   const int tok0 = tile * 16 / G, tok1 = (tile * 16 + rows - 1) / G;
   const Sight sight(r.pos + tok0, r.pos + tok1, a.window, a.first, PD_KEYS);
+
+  const uint32_t ring = smem_u32(smem) + warp * Cfg::RING;
+  const int n_mine = sight.blocks > part * W + warp ? (sight.blocks - part * W - warp + parts * W - 1) / (parts * W) : 0;
+  auto my_block = [&](int i) { return sight.block((i * parts + part) * W + warp); };
+  // a lane keeps the page of one of the next 32 blocks, so that the way over the page table is taken once for all of them
+  int page = 0;
+  auto fetch = [&](int i) {
+    if (i >= n_mine)
+      return;
+    if (i % 32 == 0 && i + lane < n_mine) {
+      page = __ldg(s.table + (size_t)seq * s.ld_table + (my_block(i + lane) * PD_KEYS >> g.page_shift));
+      if ((unsigned)page >= (unsigned)g.n_pages) {
+        atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
+        page = g.n_pages; // outside the map: zeros
+      }
+    }
+    const int from = __shfl_sync(FULL, page, i % 32), row = my_block(i) * PD_KEYS & ((1 << g.page_shift) - 1);
+    if (lane == 0) {
+      const uint32_t bar = bars + 8 * (i % Cfg::STAGES), dst = ring + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES;
+      mbar_expect_tx(bar, 2 * Cfg::KV_BYTES);
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+        tma_box4(dst + c * 2048, &kmap, 64 * c, row, h, from, bar);
+        tma_box4(dst + Cfg::KV_BYTES + c * 2048, &vmap, 64 * c, row, h, from, bar);
+      }
+    }
+  };
+  for (int i = 0; i < Cfg::STAGES - 1; ++i)
+    fetch(i);
 
   // this lane's two rows: lane / 4 and 8 more
   const int gr = lane >> 2, gc = lane & 3;
@@ -132,64 +211,31 @@ __global__ void __launch_bounds__(W * 32) paged_attention_few_kernel(AttendArgs 
       }
   }
 
-  const uint32_t ring = smem_u32(smem) + warp * Cfg::RING;
-  const int n_mine = sight.blocks > part * W + warp ? (sight.blocks - part * W - warp + parts * W - 1) / (parts * W) : 0;
-  auto my_block = [&](int i) { return sight.block((i * parts + part) * W + warp); };
-  // a lane keeps the address of one of the next 32 blocks, so that the way over the page table is taken once for all of them
-  long long at = 0;
-  constexpr int CHUNKS = HD / 8, STEP = 32 / CHUNKS; // 16-byte pieces of a row; rows that the lanes take at a time
-  const int c0 = lane % CHUNKS, r0 = lane / CHUNKS;
-  const long long pitch = (long long)g.hkv * g.hd, lane_at = r0 * pitch + 8 * c0;
-  // rows' pieces are spread over the banks for ldmatrix: piece c of a row lies at c ^ (row & 7)
-  const uint32_t lane_to = ring + r0 * (HD * 2) + ((c0 ^ r0) << 4);
-  auto fetch = [&](int i) {
-    if (i < n_mine) {
-      if (i % 32 == 0)
-        at = i + lane < n_mine ? g.row_offset(s, seq, my_block(i + lane) * PD_KEYS, h) : 0;
-      const long long off = __shfl_sync(FULL, at, i % 32);
-      const int j0 = my_block(i) * PD_KEYS;
-      if (off < 0 && lane == 0)
-        atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
-      const uint32_t dst = lane_to + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES;
-      const bool whole = off >= 0 && j0 + PD_KEYS - 1 <= sight.hi && (j0 >= sight.from || j0 + PD_KEYS <= sight.first) && 8 * c0 < g.hd;
-      const T *kp = static_cast<const T *>(a.k) + (off < 0 ? 0 : off + lane_at), *vp = static_cast<const T *>(a.v) + (off < 0 ? 0 : off + lane_at);
-#pragma unroll
-      for (int u = 0; u < PD_KEYS / STEP; ++u) {
-        const uint32_t to = (dst + u * STEP * (HD * 2)) ^ ((u * STEP & 7) << 4);
-        int bytes = 16;
-        if (!whole) {
-          const bool there = off >= 0 && sight.row_read(j0 + r0 + u * STEP) && 8 * c0 < g.hd;
-          bytes = there ? 16 : 0;
-        }
-        cp16(to, bytes ? kp : static_cast<const T *>(a.k), bytes);
-        cp16(to + Cfg::KV_BYTES, bytes ? vp : static_cast<const T *>(a.v), bytes);
-        kp += STEP * pitch;
-        vp += STEP * pitch;
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-
   float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < HD / 8; ++c)
     o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-  constexpr float LIFT = 10.f; // log2 of the factor of the probabilities
-  for (int i = 0; i < Cfg::STAGES - 1; ++i)
-    fetch(i);
+  constexpr float MOST = std::is_same<T, __half>::value ? 32768.f : 1e30f; // sum of a lane's probabilities up to which each fits its type
   for (int i = 0; i < n_mine; ++i) {
     fetch(i + Cfg::STAGES - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::STAGES - 1) : "memory");
-    __syncwarp();
+    if (!mbar_wait_warp(bars + 8 * (i % Cfg::STAGES), i / Cfg::STAGES & 1, abort_flag, &g_paged_attn_status, PD_POLLS, 2048))
+      break;
     const uint32_t kt = ring + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES, vt = kt + Cfg::KV_BYTES;
     const int j0 = my_block(i) * PD_KEYS;
+    if (!(j0 + PD_KEYS - 1 <= sight.hi && (j0 >= sight.from || j0 + PD_KEYS <= sight.first))) {
+      // rows that nobody sees meet probabilities of zero: what they hold must be finite
+      for (int k = lane; k < Cfg::KV_BYTES / 16; k += 32)
+        if (!sight.row_read(j0 + (k >> 3 & (PD_KEYS - 1))))
+          sts128(vt + 16 * k, 0, 0, 0, 0);
+      __syncwarp();
+    }
     float sc[2][4] = {}, odd[2][4] = {}; // two sums each: shorter chains
     { // four 8 x 8 matrices: keys 0-7 and 8-15, each with the lower and the upper 8 of 16 dimensions
       const int row = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
       for (int c = 0; c < HD / 16; ++c) {
         uint32_t b[4];
-        ldsm4(b, kt + row * (HD * 2) + (((2 * c + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+        ldsm4(b, kt + (c >> 2) * 2048 + row * 128 + (((2 * (c & 3) + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
         mma16816<T>(c & 1 ? odd[0] : sc[0], qf[c], b[0], b[1]);
         mma16816<T>(c & 1 ? odd[1] : sc[1], qf[c], b[2], b[3]);
       }
@@ -198,55 +244,86 @@ __global__ void __launch_bounds__(W * 32) paged_attention_few_kernel(AttendArgs 
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = j0 + 8 * t + 2 * gc + (e & 1), p = row_pos[e >> 1];
-        sc[t][e] = whole || (j <= p && (j > p - a.window || j < a.first)) ? (sc[t][e] + odd[t][e]) * a.scale_log2 : -INFINITY;
-      }
-    uint32_t pf[4];
+      for (int e = 0; e < 4; ++e)
+        sc[t][e] += odd[t][e];
+    if (!whole)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) { // the lane's two rows
-      float mx = fmaxf(fmaxf(sc[0][2 * k], sc[0][2 * k + 1]), fmaxf(sc[1][2 * k], sc[1][2 * k + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
-      mx = fmaxf(mx, m[k]);
-      const float base = mx == -INFINITY ? 0.f : mx - LIFT; // nothing seen yet: all weights are exp2(-inf)
-      const float turn = ex2(m[k] - mx); // m = mx = -inf: NaN, replaced below
-      const float keep = m[k] == mx ? 1.f : turn;
-      m[k] = mx;
-      const float p0 = ex2(sc[0][2 * k] - base), p1 = ex2(sc[0][2 * k + 1] - base), p2 = ex2(sc[1][2 * k] - base),
-                  p3 = ex2(sc[1][2 * k + 1] - base);
-      l[k] = l[k] * keep + ((p0 + p1) + (p2 + p3));
-      pf[k] = pack2<T>(p0, p1);
-      pf[k + 2] = pack2<T>(p2, p3);
-      if (__any_sync(FULL, keep != 1.f))
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          o[c][2 * k] *= keep;
-          o[c][2 * k + 1] *= keep;
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + 8 * t + 2 * gc + (e & 1), p = row_pos[e >> 1];
+          sc[t][e] = j <= p && (j > p - a.window || j < a.first) ? sc[t][e] : -INFINITY;
         }
+    uint32_t pf[4];
+    float sum[2];
+    // A row's probabilities refer to a maximum m that is taken in the first block, and where rows are masked. Other blocks go by the m there
+    // is; what they give shows whether it does. If not they begin again, with the maximum.
+    for (bool afresh = i == 0 || !whole;; afresh = true) {
+      if (afresh) {
+        float mx[2], keep[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          mx[k] = fmaxf(fmaxf(sc[0][2 * k], sc[0][2 * k + 1]), fmaxf(sc[1][2 * k], sc[1][2 * k + 1]));
+#pragma unroll
+        for (int d = 1; d < 4; d *= 2)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            mx[k] = fmaxf(mx[k], __shfl_xor_sync(FULL, mx[k], d));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float big = fmaxf(m[k], mx[k] * a.scale_log2);
+          keep[k] = big > m[k] ? ex2(m[k] - big) : 1.f;
+          m[k] = big;
+          l[k] *= keep[k];
+        }
+        if (__any_sync(FULL, keep[0] != 1.f || keep[1] != 1.f))
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c) {
+            o[c][0] *= keep[0];
+            o[c][1] *= keep[0];
+            o[c][2] *= keep[1];
+            o[c][3] *= keep[1];
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) { // the lane's two rows
+        const float base = m[k] == -INFINITY ? 0.f : m[k] - PAGED_LIFT; // nothing seen yet: all weights are 2^(-inf)
+        const float p0 = ex2(fmaf(sc[0][2 * k], a.scale_log2, -base)), p1 = ex2(fmaf(sc[0][2 * k + 1], a.scale_log2, -base)),
+                    p2 = ex2(fmaf(sc[1][2 * k], a.scale_log2, -base)), p3 = ex2(fmaf(sc[1][2 * k + 1], a.scale_log2, -base));
+        sum[k] = (p0 + p1) + (p2 + p3);
+        pf[k] = pack2<T>(p0, p1);
+        pf[k + 2] = pack2<T>(p2, p3);
+      }
+      if (afresh || !__any_sync(FULL, sum[0] > MOST || sum[1] > MOST))
+        break;
     }
+    l[0] += sum[0];
+    l[1] += sum[1];
     { // keys 0-7 and 8-15 of eight dimensions, then of the next eight
       const int row = lane & 15;
 #pragma unroll
       for (int c = 0; c < HD / 16; ++c) {
         uint32_t b[4];
-        ldsm4t(b, vt + row * (HD * 2) + (((2 * c + (lane >> 4)) ^ (row & 7)) << 4));
+        ldsm4t(b, vt + (c >> 2) * 2048 + row * 128 + (((2 * (c & 3) + (lane >> 4)) ^ (row & 7)) << 4));
         mma16816<T>(o[2 * c], pf, b[0], b[1]);
         mma16816<T>(o[2 * c + 1], pf, b[2], b[3]);
       }
     }
-    __syncwarp(); // the slot is read: the copies of the next round may fill it
+    loads_before_refill(); // the slot is read: the copies of the next round may fill it
+    __syncwarp();
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     l[k] += __shfl_xor_sync(FULL, l[k], 1);
     l[k] += __shfl_xor_sync(FULL, l[k], 2);
   }
+  if (*abort_flag) // copies in flight get time to land before the rings are used otherwise
+    for (int i = 0; i < 1000; ++i)
+      __nanosleep(1000);
 
-  /* ---- the warps' parts, then the CTAs': each a row's O, m and l; the ring is free */
+  /* ---- the warps' parts, then the CTAs': each a row's O, m and l; the rings are free */
   __syncthreads();
-  float *mine = reinterpret_cast<float *>(smem) + warp * (Cfg::PART / 4);
+  float *mine = reinterpret_cast<float *>(smem + warp * Cfg::RING);
 #pragma unroll
   for (int c = 0; c < HD / 8; ++c)
 #pragma unroll
@@ -254,83 +331,59 @@ __global__ void __launch_bounds__(W * 32) paged_attention_few_kernel(AttendArgs 
       *reinterpret_cast<float2 *>(mine + (gr + 8 * k) * HD + 8 * c + 2 * gc) = make_float2(o[c][2 * k], o[c][2 * k + 1]);
   if (gc == 0)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      mine[16 * HD + gr + 8 * k] = m[k];
-      mine[16 * HD + 16 + gr + 8 * k] = l[k];
-    }
+    for (int k = 0; k < 2; ++k)
+      *reinterpret_cast<float2 *>(mine + 16 * HD + 2 * (gr + 8 * k)) = make_float2(m[k], l[k]);
   __syncthreads();
-  // sum of n parts: part i of a value is at(i, element); returns the row's denominator by *total
-  auto joined = [&](int n, auto part_of, int row, int col, float *mx, float *total) {
-    float big = -INFINITY;
-    for (int i = 0; i < n; ++i)
-      big = fmaxf(big, part_of(i, 16 * HD + row, 1).x);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float lsum = 0.f;
-    for (int i = 0; i < n; ++i) {
-      const float mi = part_of(i, 16 * HD + row, 1).x, w = mi == -INFINITY ? 0.f : ex2(mi - big);
-      const float4 v = part_of(i, row * HD + col, 4);
-      lsum += w * part_of(i, 16 * HD + 16 + row, 1).x;
-      sum = make_float4(sum.x + w * v.x, sum.y + w * v.y, sum.z + w * v.z, sum.w + w * v.w);
-    }
-    *mx = big;
-    *total = lsum;
-    return sum;
-  };
-  constexpr int OWN = W * (Cfg::RING > Cfg::PART ? Cfg::RING : Cfg::PART); // bytes in front of the CTA's part
-  float *cta = reinterpret_cast<float *>(smem + OWN);
-  auto of_warp = [&](int i, int e, int n) {
-    const float *p = reinterpret_cast<const float *>(smem) + i * (Cfg::PART / 4) + e;
-    return n == 4 ? *reinterpret_cast<const float4 *>(p) : make_float4(*p, 0.f, 0.f, 0.f);
-  };
+  float *cta = reinterpret_cast<float *>(smem + Cfg::OFF_PART);
   const uint32_t cta_addr = smem_u32(cta);
-  auto of_cta = [&](int i, int e, int n) {
-    if (n == 4)
-      return ld_cluster4(cta_addr + 4u * e, i);
-    uint32_t remote;
-    float x;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(cta_addr + 4u * e), "r"(i));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote) : "memory");
-    return make_float4(x, 0.f, 0.f, 0.f);
-  };
-  auto store = [&](int row, int col, const float4 &sum, float mx, float total) {
+  auto store = [&](int row, int col, const Joined &j) {
     const int flat = tile * 16 + row, head = h * G + flat % G;
-    if (a.sink && mx > -INFINITY)
-      total += ex2(a.sink[head] * LOG2E - (mx - LIFT));
+    float total = j.l;
+    if (a.sink && j.m > -INFINITY)
+      total += ex2(a.sink[head] * LOG2E - (j.m - PAGED_LIFT));
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    const float4 f = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+    const float4 f = make_float4(j.sum.x * inv, j.sum.y * inv, j.sum.z * inv, j.sum.w * inv);
     const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd + col;
     if (a.out_f32)
       *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + e) = f;
     else
       *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + e) = make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
   };
-  for (int i = threadIdx.x; i < 16 * HD / 4; i += W * 32) {
+  const bool gave_up = parts == 1 && *abort_flag; // then the result stays as it is
+  for (int i = threadIdx.x; i < rows * (HD / 4); i += W * 32) {
     const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
-    if (row >= rows || col >= g.hd)
+    if (col >= g.hd)
       continue;
-    float mx, total;
-    const float4 sum = joined(W, of_warp, row, col, &mx, &total);
+    const Joined j(W, [&](int k, float4 *v, float2 *ml) {
+      const float *p = reinterpret_cast<const float *>(smem + k * Cfg::RING);
+      *v = *reinterpret_cast<const float4 *>(p + row * HD + col);
+      *ml = *reinterpret_cast<const float2 *>(p + 16 * HD + 2 * row);
+    });
     if (parts == 1) {
-      store(row, col, sum, mx, total);
+      if (!gave_up)
+        store(row, col, j);
       continue;
     }
-    *reinterpret_cast<float4 *>(cta + row * HD + col) = sum;
-    if (col == 0) {
-      cta[16 * HD + row] = mx;
-      cta[16 * HD + 16 + row] = total;
-    }
+    *reinterpret_cast<float4 *>(cta + row * HD + col) = j.sum;
+    if (col == 0)
+      *reinterpret_cast<float2 *>(cta + 16 * HD + 2 * row) = make_float2(j.m, j.l);
   }
   if (parts == 1)
     return;
   cluster_sync();
-  for (int i = part * W * 32 + threadIdx.x; i < 16 * HD / 4; i += parts * W * 32) {
-    const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
-    if (row >= rows || col >= g.hd)
-      continue;
-    float mx, total;
-    const float4 sum = joined(parts, of_cta, row, col, &mx, &total);
-    store(row, col, sum, mx, total);
-  }
+  const uint32_t raised = neighbour_raised(smem_u32(const_cast<int *>(abort_flag)), lane);
+  if (!__any_sync(FULL, raised))
+    for (int i = part * W * 32 + threadIdx.x; i < rows * (HD / 4); i += parts * W * 32) {
+      const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
+      if (col >= g.hd)
+        continue;
+      store(row, col, Joined(parts, [&](int k, float4 *v, float2 *ml) {
+              uint32_t remote;
+              *v = ld_cluster4(cta_addr + 4u * (row * HD + col), k);
+              asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(cta_addr + 4u * (16 * HD + 2 * row)), "r"(k));
+              asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(ml->x), "=f"(ml->y) : "r"(remote) : "memory");
+            }));
+    }
   cluster_sync(); // nobody leaves while its part is read
 }
 
@@ -383,7 +436,13 @@ static int launch_few(const AttendArgs &a, const PagedGeom &g, const PagedBatch 
   cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, g, s);
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const int rc = encode_map_pages(&maps[i], i ? a.v : a.k, g.hd, 1 << g.page_shift, g.hkv, g.n_pages, g.page_stride, PD_KEYS);
+    if (rc)
+      return rc;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], a, g, s);
   count_launch();
   return check_cuda(e, "paged_attention launch");
 }

@@ -29,6 +29,8 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
+/** log2 of what a row's greatest probability is when its maximum is taken */
+constexpr float PAGED_LIFT = 6.f;
 
 /* Blocks of KEYS cache rows that hold what a tile of queries at positions lo .. hi sees: those of the first tokens, then the window's.
  * A row in none of the queries' sight counts as not there: it may hold anything. */

@@ -49,7 +49,6 @@ constexpr int PC_MMA_WARP = 2 * PC_ROW_WARPS, PC_COPY_WARP = PC_MMA_WARP + 2;
 constexpr int PC_THREADS = (PC_MMA_WARP + 4) * 32; // the last warp only makes the group of four whole
 /* Registers of a thread: 96 at launch (640 * 96 of the 65536); the last group gives some to the others: 4 * 104 + 64 = 5 * 96. */
 constexpr int PC_REGS_ROWS = 104, PC_REGS_REST = 64;
-constexpr float PC_LIFT = 6.f; // log2 of what a row's greatest probability is when its maximum is taken
 constexpr uint32_t PC_POLLS = 1u << 22;
 template <int HD> struct PcCfg {
   static constexpr int TILE = 128 * HD * 2; // bytes of a tile of Q, K or V: [64 dimensions of HD][row][128 B], 128-byte swizzle
@@ -126,12 +125,6 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tma_box4(uint32_t dst, const CUtensorMap *map, int x, int row, int head, int page, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(bar)
-               : "memory");
-}
 
 template <typename T> struct MmaType;
 template <> struct MmaType<__half> {
@@ -413,7 +406,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : m - PC_LIFT;
+        const float base = m == -INFINITY ? 0.f : m - PAGED_LIFT;
         sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -457,7 +450,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       if (parts == 1) {
         float total = l;
         if (a.sink && m > -INFINITY && there)
-          total += ex2(a.sink[head] * LOG2E - (m - PC_LIFT));
+          total += ex2(a.sink[head] * LOG2E - (m - PAGED_LIFT));
         inv = total == 0.f ? 0.f : 1.f / total;
       }
       const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd;
@@ -630,7 +623,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
             f = make_float4(f.x + w * v[k].x, f.y + w * v[k].y, f.z + w * v[k].z, f.w + w * v[k].w);
           }
         if (a.sink && big > -INFINITY)
-          total += ex2(a.sink[head] * LOG2E - (big - PC_LIFT));
+          total += ex2(a.sink[head] * LOG2E - (big - PAGED_LIFT));
         const float inv = total == 0.f ? 0.f : 1.f / total;
         const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd + col;
         if (col < g.hd) {

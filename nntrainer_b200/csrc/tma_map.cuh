@@ -32,5 +32,12 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap *map, i
                : "memory");
 }
 
+/** Copies a box of a map of pages. x a multiple of 8. */
+__device__ __forceinline__ void tma_box4(uint32_t dst, const CUtensorMap *map, int x, int row, int head, int page, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(bar)
+               : "memory");
+}
+
 } // namespace nntr
 #endif

@@ -50,6 +50,14 @@ __device__ __forceinline__ void cluster_sync() {
   cluster_wait();
 }
 
+/** one lane of the warp, the same every time, in a branch that the compiler knows one lane takes: operands of copies and MMAs can be
+ *  uniform registers there (with `lane == 0` a tiled copy takes 120 clocks to issue) */
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 /* A wait that ran out in one CTA of a cluster leaves its neighbours' results without its part, so they have to know before they
  * store anything. flag: shared address of the word in which a CTA notes that it gave up, the same in every CTA. */
 /** Every thread that knows that its CTA gave up raises the neighbours' flags, before the barrier behind which the parts are used

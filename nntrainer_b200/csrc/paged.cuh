@@ -42,8 +42,8 @@ struct SeqRows {
   int first, n, pos;
   bool bad;
 };
-__device__ __forceinline__ SeqRows seq_rows(const PagedBatch &s, int b) {
-  const int lo = __ldg(s.row_start + b), hi = __ldg(s.row_start + b + 1), given = __ldg(s.context + b), ctx = min(given, s.table_rows);
+__device__ __forceinline__ SeqRows seq_rows(const PagedBatch &s, int lo, int hi, int given) { // row_start of it and of the next one, context
+  const int ctx = min(given, s.table_rows);
   SeqRows r;
   r.first = min(max(lo, 0), s.tokens);
   const int end = min(max(hi, r.first), s.tokens);
@@ -51,6 +51,9 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedBatch &s, int b) {
   r.pos = ctx - (end - r.first);
   r.bad = lo < 0 || hi < lo || hi > s.tokens || hi - lo > s.max_new || r.pos < 0 || given != ctx;
   return r;
+}
+__device__ __forceinline__ SeqRows seq_rows(const PagedBatch &s, int b) {
+  return seq_rows(s, __ldg(s.row_start + b), __ldg(s.row_start + b + 1), __ldg(s.context + b));
 }
 /** The sequence that query row `token` belongs to, by all lanes of a warp; batch where it lies behind the last one. */
 __device__ __forceinline__ int seq_of_row(const PagedBatch &s, int token, int lane) {

@@ -50,9 +50,9 @@ template <int HD, int W> struct PdCfg { // W warps
   static constexpr int STAGES = HD == 128 ? 3 : 6;
   static constexpr int KV_BYTES = PD_KEYS * HD * 2; // [64 dimensions of HD][row][128 B], 128-byte swizzle
   static constexpr int RING = STAGES * 2 * KV_BYTES; // of a warp
-  static constexpr int PART = (16 * HD + 32) * 4;    // O and (m, l) of a warp or a CTA
-  static_assert(RING >= PART && RING % 1024 == 0, "the warps' parts lie in the rings' place");
-  static constexpr int OFF_PART = W * RING, OFF_BARS = OFF_PART + PART;
+  static_assert(RING >= (16 * HD + 32) * 4 && RING % 1024 == 0, "the warps' parts, O and (m, l), lie in the rings' place");
+  // parts of the elements that a CTA joins (four columns of a row), from each of up to 16 CTAs: O, then (m, l) of each
+  static constexpr int PARTS = 16 * HD / 4 + 16, PART_ML = PARTS * 16, OFF_PART = W * RING, OFF_BARS = OFF_PART + PARTS * 24;
   static constexpr int SMEM = OFF_BARS + W * STAGES * 8 + 16;
 };
 
@@ -119,7 +119,7 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
                            PagedBatch s) {
   using Cfg = PdCfg<HD, W>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(FULL, threadIdx.x >> 5, 0);
   const int parts = cluster_size(), part = cluster_rank();
   const int tile = blockIdx.x / parts, h = blockIdx.y;
   const uint32_t bars = smem_u32(smem) + Cfg::OFF_BARS + warp * Cfg::STAGES * 8;
@@ -132,35 +132,52 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
   }
   if (threadIdx.x == 0)
     *abort_flag = 0;
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)));
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)));
+  }
+  if (parts > 1)
+    cluster_arrive(); // every CTA has started before one writes into another
   pdl_wait();
   // Long contexts begin first: of up to 128 sequences (one per thread) the one with as many longer ones as CTAs are in front
   int seq = blockIdx.z;
+  SeqRows r;
   if (s.batch > 1 && s.batch <= 128) {
-    int *rows_of = reinterpret_cast<int *>(smem), *chosen = rows_of + 128;
-    const int b = threadIdx.x, mine = b < s.batch ? __ldg(s.context + b) : 0;
+    int *rows_of = reinterpret_cast<int *>(smem);
+    int4 *chosen = reinterpret_cast<int4 *>(rows_of + 128);
+    const int b = threadIdx.x;
+    int4 mine = make_int4(b, 0, 0, INT_MIN);
+    if (b < s.batch)
+      mine = make_int4(b, __ldg(s.row_start + b), __ldg(s.row_start + b + 1), __ldg(s.context + b));
     if (b < 128)
-      rows_of[b] = b < s.batch ? mine : INT_MIN;
+      rows_of[b] = mine.w;
     __syncthreads();
     int longer = 0;
 #pragma unroll 4
     for (int i = 0; i < s.batch; i += 4) {
       const int4 v = *reinterpret_cast<const int4 *>(rows_of + i);
-      longer += (v.x > mine || (v.x == mine && i < b)) + (v.y > mine || (v.y == mine && i + 1 < b)) + (v.z > mine || (v.z == mine && i + 2 < b)) +
-                (v.w > mine || (v.w == mine && i + 3 < b));
+      longer += (v.x > mine.w || (v.x == mine.w && i < b)) + (v.y > mine.w || (v.y == mine.w && i + 1 < b)) +
+                (v.z > mine.w || (v.z == mine.w && i + 2 < b)) + (v.w > mine.w || (v.w == mine.w && i + 3 < b));
     }
     if (b < s.batch && longer == (int)blockIdx.z)
-      *chosen = b;
+      *chosen = mine;
     __syncthreads();
-    seq = *chosen;
+    const int4 it = *chosen;
+    seq = __shfl_sync(FULL, it.x, 0);
+    r = seq_rows(s, it.y, it.z, it.w);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the rings begin here
+  } else {
+    r = seq_rows(s, seq);
   }
   __syncthreads();
-  const SeqRows r = seq_rows(s, seq);
   if (r.bad && threadIdx.x == 0)
     atomicExch(&g_paged_attn_status, NNTR_CUDA_ERR_INVALID);
   const int G = g.hq / g.hkv, rows = min(16, r.n * G - tile * 16);
-  if (rows <= 0)
-    return; // every CTA of the cluster alike
+  if (rows <= 0) { // every CTA of the cluster alike
+    if (parts > 1)
+      cluster_wait();
+    return;
+  }
   const int tok0 = tile * 16 / G, tok1 = (tile * 16 + rows - 1) / G;
   const Sight sight(r.pos + tok0, r.pos + tok1, a.window, a.first, PD_KEYS);
 
@@ -180,7 +197,7 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
       }
     }
     const int from = __shfl_sync(FULL, page, i % 32), row = my_block(i) * PD_KEYS & ((1 << g.page_shift) - 1);
-    if (lane == 0) {
+    if (elected()) {
       const uint32_t bar = bars + 8 * (i % Cfg::STAGES), dst = ring + (i % Cfg::STAGES) * 2 * Cfg::KV_BYTES;
       mbar_expect_tx(bar, 2 * Cfg::KV_BYTES);
 #pragma unroll
@@ -349,42 +366,43 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
     else
       *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + e) = make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
   };
+  if (parts > 1) {
+    cluster_wait(); // for the start
+    if (*abort_flag)
+      raise_in_cluster(smem_u32(const_cast<int *>(abort_flag)));
+  }
   const bool gave_up = parts == 1 && *abort_flag; // then the result stays as it is
-  for (int i = threadIdx.x; i < rows * (HD / 4); i += W * 32) {
+  // element i of the result (four columns of a row) is joined by CTA i / share of the cluster, which gets every CTA's part of it
+  const int elements = rows * (HD / 4), share = (elements + parts - 1) / parts;
+  for (int i = threadIdx.x; i < elements; i += W * 32) {
     const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
-    if (col >= g.hd)
-      continue;
     const Joined j(W, [&](int k, float4 *v, float2 *ml) {
       const float *p = reinterpret_cast<const float *>(smem + k * Cfg::RING);
       *v = *reinterpret_cast<const float4 *>(p + row * HD + col);
       *ml = *reinterpret_cast<const float2 *>(p + 16 * HD + 2 * row);
     });
-    if (parts == 1) {
-      if (!gave_up)
-        store(row, col, j);
-      continue;
+    if (parts > 1) {
+      const int owner = i / share, at = part * share + i % share;
+      st_cluster4(cta_addr + 16u * at, owner, j.sum);
+      uint32_t remote;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(cta_addr + Cfg::PART_ML + 8u * at), "r"(owner));
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(remote), "f"(j.m), "f"(j.l) : "memory");
+    } else if (col < g.hd && !gave_up) {
+      store(row, col, j);
     }
-    *reinterpret_cast<float4 *>(cta + row * HD + col) = j.sum;
-    if (col == 0)
-      *reinterpret_cast<float2 *>(cta + 16 * HD + 2 * row) = make_float2(j.m, j.l);
   }
   if (parts == 1)
     return;
-  cluster_sync();
-  const uint32_t raised = neighbour_raised(smem_u32(const_cast<int *>(abort_flag)), lane);
-  if (!__any_sync(FULL, raised))
-    for (int i = part * W * 32 + threadIdx.x; i < rows * (HD / 4); i += parts * W * 32) {
-      const int row = i / (HD / 4), col = 4 * (i % (HD / 4));
-      if (col >= g.hd)
-        continue;
-      store(row, col, Joined(parts, [&](int k, float4 *v, float2 *ml) {
-              uint32_t remote;
-              *v = ld_cluster4(cta_addr + 4u * (row * HD + col), k);
-              asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(cta_addr + 4u * (16 * HD + 2 * row)), "r"(k));
-              asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(ml->x), "=f"(ml->y) : "r"(remote) : "memory");
-            }));
+  cluster_sync(); // behind it nobody touches another's memory
+  if (!*abort_flag)
+    for (int k = threadIdx.x; k < share && part * share + k < elements; k += W * 32) {
+      const int i = part * share + k, row = i / (HD / 4), col = 4 * (i % (HD / 4));
+      if (col < g.hd)
+        store(row, col, Joined(parts, [&](int q, float4 *v, float2 *ml) {
+                *v = *reinterpret_cast<const float4 *>(cta + 4 * (q * share + k));
+                *ml = *reinterpret_cast<const float2 *>(reinterpret_cast<const uint8_t *>(cta) + Cfg::PART_ML + 8 * (q * share + k));
+              }));
     }
-  cluster_sync(); // nobody leaves while its part is read
 }
 
 /* ------------------------------------------------------------------ launch */

@@ -739,12 +739,12 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     if top_k < 0:
         raise ValueError("top_k is a count")
     rows = logits.numel() // n if n else 0
-    if idx is None and idx_f is None and prob is None:  # one allocation
-        idx, idx_f, prob = torch.empty((3, rows), dtype=f32, device=logits.device).unbind()
-        idx = idx.view(torch.int32)
-    else:
-        new = lambda t, dt: torch.empty(rows, dtype=dt, device=logits.device) if t is None else t  # noqa: E731
-        idx, idx_f, prob = new(idx, torch.int32), new(idx_f, f32), new(prob, f32)
+    if idx is None:
+        idx = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    if idx_f is None:
+        idx_f = torch.empty_like(idx, dtype=f32)
+    if prob is None:
+        prob = torch.empty_like(idx_f)
     rc = lib().nntr_cuda_sample_dev(
         logits.data_ptr(), rows, n, stride[0] if len(shape) == 2 else n, _typed(u, "u", f32, rows), temperature, top_k, top_p, min_p,
         _typed(params, "params", f32, 4 * rows), _typed(idx, "out", torch.int32, rows), _typed(idx_f, "out", f32, rows),

@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     temperature = p[0] <= 1e30f ? p[0] : p[0] > 0.f ? 1e30f : 0.f, top_p = p[2], min_p = p[3];
     top_k = p[1] >= 1.f ? (unsigned)fminf(p[1], 1e9f) : 0u;
   }
-  // this warp's slice of the row
-  const unsigned s0 = min(a.n, (unsigned)(part * SP_WARPS + warp) * a.sub_len), s1 = min(a.n, s0 + a.sub_len);
+  // this warp's slice of the row: the CTAs take slices in turn, so that none has all of the tokens that a model likes (low indices, often)
+  const unsigned sub = warp * parts + part, s0 = min(a.n, sub * a.sub_len), s1 = min(a.n, s0 + a.sub_len);
   constexpr int AT = 4; // loads of a lane on their way at a time
   auto for_slice = [&](auto f) { // f(index, four logits); what is behind the slice is NaN
     for (unsigned i0 = s0 + 4 * lane; i0 - 4 * lane < s1; i0 += 128 * AT) {
@@ -364,24 +364,38 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
   auto bin_of = [&](float v) { return min(SP_BINS - 1, (int)fminf((mx - v) * per_bin, (float)SP_BINS)); };
   auto edge_of = [&](int bin) { return bin >= SP_BINS ? -3.402823466e38f : mx - (float)bin / per_bin; }; // the least value of the bins in front
   float head = -3.402823466e38f;
+  const unsigned wanted = has_k ? min((unsigned)SP_HEAD, 2 * min(top_k, (unsigned)SP_HEAD) + 32) : SP_HEAD;
   if (a.n > SP_LIST) {
     sh.bins[tid] = 0;
     __syncthreads();
-    for (unsigned i0 = s0 + (part * SP_WARPS + warp) % SP_EVERY * 128; i0 < s1; i0 += 128 * SP_EVERY)
+    for (unsigned i0 = s0 + sub % SP_EVERY * 128; i0 < s1; i0 += 128 * SP_EVERY * 4) {
+      float v[4][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const unsigned i = i0 + 32 * k + lane;
-        const float v = i < s1 ? x[i] : NAN;
-        if (v > -INFINITY)
-          atomicAdd(&sh.bins[bin_of(v)], 1u);
-      }
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned i = i0 + 128 * SP_EVERY * b + 32 * k + lane;
+          v[b][k] = i < s1 ? x[i] : NAN;
+        }
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (v[b][k] > -INFINITY)
+            atomicAdd(&sh.bins[bin_of(v[b][k])], 1u);
+    }
     __syncthreads();
     uint32_t all = sh.bins[tid];
     if (parts > 1) {
       cluster_sync();
+      uint32_t of[SP_MAX_PARTS];
+#pragma unroll
+      for (int k = 0; k < SP_MAX_PARTS; ++k)
+        of[k] = k < parts ? ld_remote32(&sh.bins[tid], k) : 0;
       all = 0;
-      for (int k = 0; k < parts; ++k)
-        all += ld_remote32(&sh.bins[tid], k);
+#pragma unroll
+      for (int k = 0; k < SP_MAX_PARTS; ++k)
+        all += of[k];
     }
     sh.all_bins[tid] = all;
     __syncthreads();
@@ -395,7 +409,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
 #pragma unroll
       for (int k = 0; k < SP_BINS / 32; ++k) {
         in_front += v[k];
-        if (in_front * SP_EVERY <= SP_HEAD)
+        if (in_front * SP_EVERY <= wanted)
           last = lane * (SP_BINS / 32) + k + 1;
       }
       last = __reduce_max_sync(FULL, last);
@@ -404,93 +418,106 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     }
     __syncthreads();
     head = sh.from;
-    if (weight.fp32)
-      weight.exact_from = fmaxf(weight.exact_from, head);
   } else {
     __syncthreads();
   }
   const float min_x = sh.min_x;
+  if (min_p > 0.0 && !(has_k && has_p)) // what is below fails min_p (top_k and top_p together refer to a sum that has it)
+    head = fmaxf(head, min_x);
+  if (weight.fp32)
+    weight.exact_from = fmaxf(weight.exact_from, head);
 
-  /* Logits from `from` up to `below` into the list, which the first CTA gets; the others, four at a time, to f(logits, for each whether it is
-   * in the list); what f adds up in each slice goes to sh.sub of the first CTA. Returns how many are listed, ~0 if they are too many. */
+  /* Logits from `from` up to `below` into the list of the first CTA; the others, four at a time, to f(logits, for each whether it is in
+   * the list); what f adds up in each slice goes to sh.sub of the first CTA. Returns how many are listed, ~0 if they are too many. Each CTA
+   * has its own part of the list. */
   unsigned long long slice_sum = 0;
   unsigned n_above = 0;
+  const unsigned room = SP_LIST / parts;
   auto gather = [&](float from, float below, auto f) {
     if (tid == 0)
       sh.count = sh.n_above = 0;
     slice_sum = 0;
     n_above = 0;
     __syncthreads();
+    uint32_t to_x, to_i;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to_x) : "r"(smem_u32(&sh.x[part * room])));
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to_i) : "r"(smem_u32(&sh.i[part * room])));
     for_slice([&](unsigned i, const float(&v)[4]) {
       bool in[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         in[k] = v[k] >= from && v[k] < below;
       f(v, in);
-      if (__any_sync(FULL, in[0] || in[1] || in[2] || in[3])) {
-        const unsigned mine = in[0] + in[1] + in[2] + in[3];
-        unsigned upto = mine; // of the lanes so far
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-          const unsigned t = __shfl_up_sync(FULL, upto, o);
-          upto += lane >= o ? t : 0;
-        }
-        unsigned at = 0;
-        if (lane == 31)
-          at = atomicAdd(&sh.count, upto);
-        at = __shfl_sync(FULL, at, 31) + upto - mine;
+      if (in[0] || in[1] || in[2] || in[3])
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (in[k]) {
-            if (at < SP_LIST) {
-              sh.x[at] = v[k];
-              sh.i[at] = i + k;
+            const unsigned at = atomicAdd(&sh.count, 1u);
+            if (at < room) {
+              asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to_x + 4 * at), "f"(v[k]) : "memory");
+              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to_i + 4 * at), "r"(i + k) : "memory");
             }
-            ++at;
           }
-      }
     });
     slice_sum = warp_sum(slice_sum);
     n_above = __reduce_add_sync(FULL, n_above);
     if (lane == 0 && n_above)
       atomicAdd(&sh.n_above, n_above);
-    __syncthreads();
-    const unsigned own = sh.count;
-    unsigned all = own;
-    if (parts == 1) {
+    if (parts > 1) {
       if (lane == 0)
-        sh.sub[warp] = slice_sum;
-      if (tid == 0)
-        sh.above[0] = sh.n_above;
-    } else {
+        st_remote64(&sh.sub[sub], 0, slice_sum);
+      __syncthreads();
       if (tid < parts) {
-        st_remote32(&sh.counts[part], tid, own);
+        st_remote32(&sh.counts[part], tid, sh.count);
         st_remote32(&sh.above[part], tid, sh.n_above);
       }
+      cluster_sync();
+    } else {
       if (lane == 0)
-        st_remote64(&sh.sub[part * SP_WARPS + warp], 0, slice_sum);
-      cluster_sync();
-      unsigned in_front = 0;
-      all = 0;
-      for (int k = 0; k < parts; ++k) {
-        in_front += k < part ? sh.counts[k] : 0;
-        all += sh.counts[k];
+        sh.sub[sub] = slice_sum;
+      __syncthreads();
+      if (tid == 0) {
+        sh.counts[0] = sh.count;
+        sh.above[0] = sh.n_above;
       }
-      if (all <= SP_LIST && part > 0)
-        for (unsigned i = tid; i < own; i += SP_THREADS) {
-          st_remote32(&sh.x[in_front + i], 0, __float_as_uint(sh.x[i]));
-          st_remote32(&sh.i[in_front + i], 0, sh.i[i]);
-        }
-      cluster_sync();
+      __syncthreads();
     }
-    if (part == 0 && all <= SP_LIST) {
-      if (parts == 1)
+    unsigned all = 0, most = 0, count[SP_MAX_PARTS];
+#pragma unroll
+    for (int k = 0; k < SP_MAX_PARTS; ++k) {
+      count[k] = k < parts ? sh.counts[k] : 0;
+      all += count[k];
+      most = max(most, count[k]);
+    }
+    if (most > room)
+      return ~0u;
+    if (part == 0) { // the parts close up: an entry moves to a place that is not behind it, so that no later one is written over
+      for (unsigned i0 = 0; i0 < (parts > 1 ? all : 0); i0 += SP_THREADS) {
+        const unsigned i = i0 + tid;
+        unsigned from_k = 0, in_front = 0;
+#pragma unroll
+        for (int k = 0; k < SP_MAX_PARTS; ++k)
+          if (i >= in_front + count[k] && i < all) {
+            in_front += count[k];
+            from_k = k + 1;
+          } else {
+            break;
+          }
+        const unsigned at = from_k * room + i - in_front;
+        const float xv = i < all ? sh.x[at] : 0.f;
+        const uint32_t iv = i < all ? sh.i[at] : 0;
         __syncthreads();
+        if (i < all) {
+          sh.x[i] = xv;
+          sh.i[i] = iv;
+        }
+      }
+      __syncthreads();
       for (unsigned i = tid; i < all; i += SP_THREADS)
         sh.w[i] = weight(sh.x[i]);
       __syncthreads();
     }
-    return all <= SP_LIST ? all : ~0u;
+    return all;
   };
 
   /* ---- the greatest logits listed, the others summed */
@@ -672,17 +699,54 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     const int n = (int)sh.few;
     if (n > SP_FEW)
       return false;
+    if (n <= 32) { // within a warp
+      if (warp > 0)
+        return true;
+      const bool there = lane < n;
+      const uint32_t o = there ? sh.few_o[lane] : 0, id = there ? sh.few_i[lane] : 0;
+      const unsigned long long w = there ? sh.few_w[lane] : 0;
+      unsigned rank = 0;
+      unsigned long long in_front = 0;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t oj = __shfl_sync(FULL, o, j), ij = __shfl_sync(FULL, id, j);
+        const unsigned long long wj = __shfl_sync(FULL, w, j);
+        const bool before = oj > o || (oj == o && ij < id);
+        rank += before;
+        in_front += before ? wj : 0;
+      }
+      bool mine = there && (!has_k || rank < top_k);
+      if (has_p) {
+        if (has_k)
+          all = warp_sum(mine ? w : 0);
+        mine = mine && in_front < (unsigned long long)ceil(top_p * (double)all);
+      }
+      mine = mine && o >= passes;
+      const unsigned long long held = mine ? w : 0;
+      unsigned long long upto = 0;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t ij = __shfl_sync(FULL, id, j);
+        const unsigned long long wj = __shfl_sync(FULL, held, j);
+        upto += ij <= id ? wj : 0;
+      }
+      const unsigned long long total = warp_sum(held), goal = goal_of(total);
+      if (held && upto >= goal && upto - held < goal)
+        tell(id, weight.exactly(value_of(o)) * SP_ONE / (double)total);
+      return true;
+    }
     const bool there = tid < n;
     const uint32_t o = there ? sh.few_o[tid] : 0, id = there ? sh.few_i[tid] : 0;
     const unsigned long long w = there ? sh.few_w[tid] : 0;
     unsigned rank = 0;
     unsigned long long in_front = 0;
     if (warp * 32 < n)
-      for (int j = 0; j < n; ++j)
-        if (sh.few_o[j] > o || (sh.few_o[j] == o && sh.few_i[j] < id)) {
-          ++rank;
-          in_front += sh.few_w[j];
-        }
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const uint32_t oj = sh.few_o[j], ij = sh.few_i[j];
+        const unsigned long long wj = sh.few_w[j];
+        const bool before = oj > o || (oj == o && ij < id);
+        rank += before;
+        in_front += before ? wj : 0;
+      }
     bool mine = there && (!has_k || rank < top_k);
     if (has_p) {
       if (has_k)
@@ -696,8 +760,12 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     const unsigned long long total = cta_sum(sh, mine ? w : 0), goal = goal_of(total);
     if (warp * 32 < n && __any_sync(FULL, mine)) {
       unsigned long long upto = 0;
-      for (int j = 0; j < n; ++j)
-        upto += sh.few_i[j] <= id ? sh.few_w[j] : 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const uint32_t ij = sh.few_i[j];
+        const unsigned long long wj = sh.few_w[j];
+        upto += ij <= id ? wj : 0;
+      }
       if (mine && w && upto >= goal && upto - w < goal)
         tell(id, weight.exactly(value_of(o)) * SP_ONE / (double)total);
     }
@@ -725,27 +793,27 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     }
     const uint32_t least = min_x >= head ? order_of(min_x) : 1u; // what lies below fails min_p
     bool enough = !deep_k;
-    if (has_k && top_k < listed)
-      cut_by_count(head, top_k);
     unsigned long long sum = 0;
     if (has_p && !has_k) {
       sum = list_sum([](unsigned, float) { return true; }) + slices_sum();
       target = (unsigned long long)ceil(top_p * (double)sum);
     }
-    bool done = false;
-    if (enough && (of_cut || least > 1u)) {
-      if (open && least > 1u)
-        say(0); // whatever top_p says, the kept tokens are listed
-      done = among_few(least, sum);
-    }
-    if (done)
+    const bool early = open && least > 1u && !deep_k; // whatever top_p says, the kept tokens are listed
+    if (early)
+      say(0);
+    if (enough && (!has_p || has_k || least > 1u || all_listed) && among_few(least, sum))
       return;
+    if (has_k && top_k < listed) {
+      cut_by_count(head, top_k);
+      if (among_few(least, sum))
+        return;
+    }
     if (has_p && enough) {
       if (has_k) {
         sum = list_sum([&](unsigned, float v) { return !of_cut || order_of(v) > cut; }) + of_cut * weight(value_of(cut));
         target = (unsigned long long)ceil(top_p * (double)sum);
       }
-      enough = cut_by_weight(head, 0, target);
+      enough = cut_by_weight(head, 0, target) || least > 1u; // what passes min_p is listed, and in front of any cut further down
       if (!enough) { // about where it is: so much of the weight that is not listed lies in front of it
         const unsigned long long rest = slices_sum();
         if (warp == 0) {
@@ -792,8 +860,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
         sh.digit = lane * (SP_BINS / 32) + k;
       }
     }
-    if (least > 1u) // what passes min_p is listed, and in front of any cut further down
-      enough = true;
+    enough = enough || least > 1u;
     __syncthreads();
     if (!enough && tid == 0) { // the bins around that one
       const unsigned half = SP_AROUND / 2 / SP_EVERY;
@@ -806,7 +873,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
       sh.from = edge_of(lo);
     }
     word = enough ? 0 : 1;
-    if (open && !(least > 1u && !deep_k))
+    if (open && !early)
       say(word);
     if (word == 0) {
       if (of_cut && among_few(least, sum))
@@ -898,11 +965,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     sum = warp_sum(sum);
     if (parts > 1) { // in every CTA
       if (lane < parts)
-        st_remote64(&sh.sub[part * SP_WARPS + warp], lane, sum);
+        st_remote64(&sh.sub[sub], lane, sum);
       cluster_sync();
     } else {
       if (lane == 0)
-        sh.sub[warp] = sum;
+        sh.sub[sub] = sum;
       __syncthreads();
     }
     return slices_sum();

@@ -653,8 +653,9 @@ def paged_append(q, k, v, kcache, vcache, page_table, row_start, context, max_ne
     if q.dtype is not f32 or k.dtype is not f32 or v.dtype is not f32 or v.stride() != ld_kv or ld[1] != 1 or ld_kv[1] != 1:
         raise ValueError("q, k and v: fp32 rows; those of k and v at the same distance")
     rows = cos.shape
-    if len(rows) != 2 or sin.shape != rows or rows[1] != hd:
-        raise ValueError("cos and sin: [positions, head_dim]")
+    if (len(rows) != 2 or sin.shape != rows or rows[1] != hd or cos.dtype is not f32 or sin.dtype is not f32 or not cos.is_contiguous()
+            or not sin.is_contiguous()):
+        raise ValueError("cos and sin: contiguous fp32 [positions, head_dim]")
     hq = width // hd
     c, b, _ = _paged(torch, kcache, vcache, hq, page_table, row_start, context, tokens, max_new, 0)
     if q_out is None:
@@ -665,7 +666,7 @@ def paged_append(q, k, v, kcache, vcache, page_table, row_start, context, max_ne
             raise ValueError("q_out: [tokens, n_heads_q, head_dim] in the caches' type")
     rc = lib().nntr_cuda_paged_append_dev(
         c, b, q.data_ptr(), k.data_ptr(), v.data_ptr(), ld[0], ld_kv[0], _typed(qg, "q_gamma", f32, hd), _typed(kg, "k_gamma", f32, hd), eps,
-        _typed(cos, "cos", f32), _typed(sin, "sin", f32), rows[0], q_out.data_ptr(), ld_out, capi.GEMV_PDL if pdl else 0, _stream())
+        cos.data_ptr(), sin.data_ptr(), rows[0], q_out.data_ptr(), ld_out, capi.GEMV_PDL if pdl else 0, _stream())
     if rc:
         check(rc)
     return q_out
@@ -697,7 +698,8 @@ def paged_attention(q, kcache, vcache, page_table, row_start, context, max_new: 
             raise ValueError("out: [tokens, n_heads_q, head_dim] in the caches' type or fp32")
         dtype = capi.F32 if out.dtype is torch.float32 else dtype
     rc = lib().nntr_cuda_paged_attention_dev(
-        c, b, q.data_ptr(), ld[0], 0xFFFFFFFF if window is None else window, first_tokens, _typed(sink, "sink", torch.float32, hq),
+        c, b, q.data_ptr(), ld[0], 0xFFFFFFFF if window is None else window, first_tokens,
+        None if sink is None else _typed(sink, "sink", torch.float32, hq),
         out.data_ptr(), dtype, ld_out, capi.GEMV_PDL if pdl else 0, _stream())
     if rc:
         check(rc)
@@ -739,16 +741,24 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     if top_k < 0:
         raise ValueError("top_k is a count")
     rows = logits.numel() // n if n else 0
+    if u.dtype is not f32 or u.numel() != rows or not u.is_contiguous():
+        raise ValueError(f"u: need a contiguous fp32 tensor of {rows} elements")
     if idx is None:
         idx = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    else:
+        _typed(idx, "out", torch.int32, rows)
     if idx_f is None:
         idx_f = torch.empty_like(idx, dtype=f32)
+    else:
+        _typed(idx_f, "out", f32, rows)
     if prob is None:
         prob = torch.empty_like(idx_f)
+    else:
+        _typed(prob, "out", f32, rows)
     rc = lib().nntr_cuda_sample_dev(
-        logits.data_ptr(), rows, n, stride[0] if len(shape) == 2 else n, _typed(u, "u", f32, rows), temperature, top_k, top_p, min_p,
-        _typed(params, "params", f32, 4 * rows), _typed(idx, "out", torch.int32, rows), _typed(idx_f, "out", f32, rows),
-        _typed(prob, "out", f32, rows), capi.GEMV_PDL if pdl else 0, _stream())
+        logits.data_ptr(), rows, n, stride[0] if len(shape) == 2 else n, u.data_ptr(), temperature, top_k, top_p, min_p,
+        None if params is None else _typed(params, "params", f32, 4 * rows), idx.data_ptr(), idx_f.data_ptr(), prob.data_ptr(),
+        capi.GEMV_PDL if pdl else 0, _stream())
     if rc:
         check(rc)
     return idx, idx_f, prob

@@ -11,6 +11,8 @@
  */
 #include "paged.cuh"
 
+#include <algorithm>
+
 namespace nntr {
 
 __device__ int g_paged_cache_status = 0;
@@ -72,81 +74,105 @@ struct AppendArgs {
   void *q_out, *kcache, *vcache;
   long long ld_q, ld_kv, ld_out;
   float eps;
-  int table_rows, vec, chunks; // vec: rows are 16-byte aligned; chunks: CTAs of a token
+  int table_rows, chunks; // chunks: CTAs of a token
 };
 
-__device__ __forceinline__ float4 load4(const float *p, int vec) {
+__device__ __forceinline__ float4 load4(const float *p, bool vec) {
   return vec ? *reinterpret_cast<const float4 *>(p) : make_float4(p[0], p[1], p[2], p[3]);
 }
 template <typename T> __device__ __forceinline__ void store4(T *p, const float4 &f) {
   *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
 }
 
-/* A CTA takes 16 heads of one token (query heads, then key heads, then value heads), 16 lanes a head. */
-template <typename T>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(AppendArgs a, PagedGeom g, PagedBatch s) {
+/* A CTA takes 16 U heads (query heads, then key heads, then value heads) of tokens that follow each other, 16 lanes a head, each lane group U
+ * heads whose loads are on their way together, before it is looked up where the token belongs. Many tokens are bound by bandwidth, if only
+ * few instructions go into an element: what a head's lanes need to know of it is computed once, mean and root by a multiplication and the
+ * approximate reciprocal root (2^-22). VEC: rows, gammas and tables are 16-byte aligned. */
+template <typename T, int U, bool VEC>
+__global__ void __launch_bounds__(PA_THREADS, U == 1 ? 5 : 4) paged_append_kernel(AppendArgs a, PagedGeom g, PagedBatch s) {
   pdl_launch_dependents();
-  pdl_wait();
   const int lane = threadIdx.x & 31, l = threadIdx.x % PA_LANES;
-  const int token = blockIdx.x / a.chunks, head = (blockIdx.x % a.chunks) * PA_HEADS + threadIdx.x / PA_LANES;
-  const int seq = seq_of_row(s, token, lane);
-  if (seq >= s.batch)
-    return; // behind the last sequence: left as it is
-  const SeqRows r = seq_rows(s, seq);
-  const int i = token - r.first, pos = r.pos + i;
-  if (r.bad && threadIdx.x == 0)
-    atomicExch(&g_paged_cache_status, NNTR_CUDA_ERR_INVALID);
-  if (i < 0 || i >= r.n || head >= g.hq + 2 * g.hkv)
-    return;
+  const int ctas = gridDim.x / a.chunks, cta = blockIdx.x / a.chunks, head0 = (blockIdx.x % a.chunks) * (PA_HEADS * U) + threadIdx.x / PA_LANES;
   const int half = g.hd / 2, e = 4 * l;
-  const bool on = e < half;
-  const int kind = head < g.hq ? 0 : head < g.hq + g.hkv ? 1 : 2, h = kind == 0 ? head : (head - g.hq) % g.hkv;
-  const float *src = kind == 0 ? a.q + token * a.ld_q : (kind == 1 ? a.k : a.v) + token * a.ld_kv;
-  src += (size_t)h * g.hd;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-  if (on) {
-    x = load4(src + e, a.vec);
-    y = load4(src + half + e, a.vec);
-  }
-  const bool placed = pos >= 0 && pos < a.table_rows; // a row of the rotation tables
-  if (kind < 2) {
-    const float *gamma = kind == 0 ? a.q_gamma : a.k_gamma;
-    if (gamma) {
-      float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + (y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
+  const float *src[U], *gamma[U];
+  T *to[U]; // row 0 of the caches or of the result
+  long long ld[U];
+  bool turned[U], query[U], on[U];
 #pragma unroll
-      for (int o = PA_LANES / 2; o; o >>= 1)
-        sum += __shfl_xor_sync(0xffffu << (lane & PA_LANES), sum, o, PA_LANES); // the head's lanes are here, the other head's may not
-      const float scale = 1.0f / sqrtf(sum / (float)g.hd + a.eps);
-      if (on) {
-        const float4 gx = load4(gamma + e, 0), gy = load4(gamma + half + e, 0);
-        x = make_float4(x.x * scale * gx.x, x.y * scale * gx.y, x.z * scale * gx.z, x.w * scale * gx.w);
-        y = make_float4(y.x * scale * gy.x, y.y * scale * gy.y, y.z * scale * gy.z, y.w * scale * gy.w);
+  for (int u = 0; u < U; ++u) {
+    const int head = head0 + u * PA_HEADS;
+    query[u] = head < g.hq;
+    turned[u] = head < g.hq + g.hkv;
+    on[u] = head < g.hq + 2 * g.hkv && e < half;
+    const int off = (query[u] ? head : turned[u] ? head - g.hq : head - g.hq - g.hkv) * g.hd + e;
+    src[u] = (query[u] ? a.q : turned[u] ? a.k : a.v) + off;
+    to[u] = static_cast<T *>(query[u] ? a.q_out : turned[u] ? a.kcache : a.vcache) + off;
+    gamma[u] = query[u] ? a.q_gamma : a.k_gamma;
+    ld[u] = query[u] ? a.ld_q : a.ld_kv;
+  }
+  const float per_dim = 1.0f / (float)g.hd;
+  pdl_wait();
+  int seq = 0;
+  SeqRows r = {0, 0, 0, false};
+  const int last = (int)((long long)s.tokens * (cta + 1) / ctas);
+  for (int token = (int)((long long)s.tokens * cta / ctas); token < last; ++token) {
+    float4 x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = y[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (on[u]) {
+        const float *p = src[u] + token * ld[u];
+        x[u] = load4(p, VEC);
+        y[u] = load4(p + half, VEC);
       }
     }
-    if (on && placed) {
-      const float4 c = load4(a.cos_tab + (size_t)pos * g.hd + e, 0), n = load4(a.sin_tab + (size_t)pos * g.hd + e, 0);
-      const float4 p = x, t = y;
-      x = make_float4(p.x * c.x - t.x * n.x, p.y * c.y - t.y * n.y, p.z * c.z - t.z * n.z, p.w * c.w - t.w * n.w);
-      y = make_float4(p.x * n.x + t.x * c.x, p.y * n.y + t.y * c.y, p.z * n.z + t.z * c.z, p.w * n.w + t.w * c.w);
+    if (token >= r.first + r.n) { // another sequence than the token's in front
+      seq = seq_of_row(s, token, lane);
+      if (seq >= s.batch)
+        return; // behind the last sequence: left as it is
+      r = seq_rows(s, seq);
+      if (r.bad && threadIdx.x == 0)
+        atomicExch(&g_paged_cache_status, NNTR_CUDA_ERR_INVALID);
     }
-  }
-  if (!on)
-    return;
-  if (!placed) // no rotation is known for it: the query is zero, no row is stored
-    x = y = make_float4(0.f, 0.f, 0.f, 0.f);
-  T *dst;
-  if (kind == 0) {
-    dst = static_cast<T *>(a.q_out) + token * a.ld_out + (size_t)h * g.hd;
-  } else {
-    const long long at = placed ? g.row_offset(s, seq, pos, h) : -1;
-    if (at < 0) {
+    const int i = token - r.first, pos = r.pos + i;
+    if (i < 0 || i >= r.n)
+      continue;
+    const bool placed = pos >= 0 && pos < a.table_rows; // a row of the rotation tables
+    const long long row = placed ? g.row_offset(s, seq, pos, 0) : -1;
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f), n = c; // no rotation is known: the query is zero, no row is stored
+    if (placed && e < half) {
+      c = load4(a.cos_tab + (size_t)pos * g.hd + e, VEC);
+      n = load4(a.sin_tab + (size_t)pos * g.hd + e, VEC);
+    }
+    if (row < 0 && l == 0)
       atomicExch(&g_paged_cache_status, NNTR_CUDA_ERR_INVALID);
-      return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (a.q_gamma) { // all lanes, whatever their heads are: a sum over lanes that not all of a warp may come to costs as much again
+        float sum = x[u].x * x[u].x + x[u].y * x[u].y + x[u].z * x[u].z + x[u].w * x[u].w +
+                    (y[u].x * y[u].x + y[u].y * y[u].y + y[u].z * y[u].z + y[u].w * y[u].w);
+#pragma unroll
+        for (int o = PA_LANES / 2; o; o >>= 1)
+          sum += __shfl_xor_sync(FULL, sum, o);
+        if (turned[u] && on[u]) {
+          const float scale = rsqrtf(fmaf(sum, per_dim, a.eps));
+          const float4 gx = load4(gamma[u] + e, VEC), gy = load4(gamma[u] + half + e, VEC);
+          x[u] = make_float4(x[u].x * scale * gx.x, x[u].y * scale * gx.y, x[u].z * scale * gx.z, x[u].w * scale * gx.w);
+          y[u] = make_float4(y[u].x * scale * gy.x, y[u].y * scale * gy.y, y[u].z * scale * gy.z, y[u].w * scale * gy.w);
+        }
+      }
+      if (turned[u]) {
+        const float4 p = x[u], t = y[u];
+        x[u] = make_float4(p.x * c.x - t.x * n.x, p.y * c.y - t.y * n.y, p.z * c.z - t.z * n.z, p.w * c.w - t.w * n.w);
+        y[u] = make_float4(p.x * n.x + t.x * c.x, p.y * n.y + t.y * c.y, p.z * n.z + t.z * c.z, p.w * n.w + t.w * c.w);
+      }
+      if (on[u] && (query[u] || row >= 0)) {
+        T *dst = to[u] + (query[u] ? token * a.ld_out : row);
+        store4(dst, x[u]);
+        store4(dst + half, y[u]);
+      }
     }
-    dst = static_cast<T *>(kind == 1 ? a.kcache : a.vcache) + at;
   }
-  store4(dst + e, x);
-  store4(dst + half + e, y);
 }
 
 static void launch_cfg(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, unsigned flags, cudaStream_t st) {
@@ -177,19 +203,29 @@ int launch_paged_append(const nntr_paged_cache *c, const nntr_paged_batch *b, co
                      (long long)ld_q, (long long)ld_kv, (long long)ld_out);
   if (table_rows > 0x7fffffffu)
     table_rows = 0x7fffffffu;
-  AppendArgs a = {q, k, v, q_gamma, k_gamma, cos_tab, sin_tab, q_out, c->kcache, c->vcache, ld_q, ld_kv, ld_out, eps, (int)table_rows, 0, 0};
-  const uintptr_t low = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
-  a.vec = !(low & 15) && ld_q % 4 == 0 && ld_kv % 4 == 0;
-  a.chunks = (g.hq + 2 * g.hkv + PA_HEADS - 1) / PA_HEADS;
-  if ((long long)s.tokens * a.chunks > 0x7fffffffll)
-    return set_error(NNTR_CUDA_ERR_UNSUPPORTED, "paged_append: too many rows in one call");
+  AppendArgs a = {q, k, v, q_gamma, k_gamma, cos_tab, sin_tab, q_out, c->kcache, c->vcache, ld_q, ld_kv, ld_out, eps, (int)table_rows, 0};
+  uintptr_t low = 0;
+  for (const float *p : {q, k, v, q_gamma, k_gamma, cos_tab, sin_tab})
+    low |= reinterpret_cast<uintptr_t>(p);
+  const bool vec = !(low & 15) && ld_q % 4 == 0 && ld_kv % 4 == 0;
+  // Heads of a lane group: one while that many CTAs do not fill the machine twice. CTAs: no more than run at a time, each with tokens
+  // that follow each other, which mostly belong to one sequence.
+  const int groups = (g.hq + 2 * g.hkv + PA_HEADS - 1) / PA_HEADS;
+  const int each = (long long)s.tokens * groups < 16ll * sm_count() ? 1 : groups % 3 == 0 || groups > 4 ? 3 : groups % 2 == 0 ? 2 : groups;
+  a.chunks = (groups + each - 1) / each;
+  const int at_once = (each == 1 ? 5 : 4) * sm_count(), ctas = std::min(s.tokens, std::max(1, at_once / a.chunks));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   launch_cfg(cfg, attr, flags, st);
-  cfg.gridDim = dim3((unsigned)(s.tokens * a.chunks));
+  cfg.gridDim = dim3((unsigned)(ctas * a.chunks));
   cfg.blockDim = dim3(PA_THREADS);
-  const cudaError_t e = c->dtype == NNTR_F16 ? cudaLaunchKernelEx(&cfg, paged_append_kernel<__half>, a, g, s)
-                                             : cudaLaunchKernelEx(&cfg, paged_append_kernel<__nv_bfloat16>, a, g, s);
+  auto launch = [&](auto value) {
+    using T = decltype(value);
+    if (!vec)
+      return cudaLaunchKernelEx(&cfg, each == 1 ? paged_append_kernel<T, 1, false> : each == 2 ? paged_append_kernel<T, 2, false> : paged_append_kernel<T, 3, false>, a, g, s);
+    return cudaLaunchKernelEx(&cfg, each == 1 ? paged_append_kernel<T, 1, true> : each == 2 ? paged_append_kernel<T, 2, true> : paged_append_kernel<T, 3, true>, a, g, s);
+  };
+  const cudaError_t e = c->dtype == NNTR_F16 ? launch(__half()) : launch(__nv_bfloat16());
   count_launch();
   return check_cuda(e, "paged_append launch");
 }

@@ -56,7 +56,8 @@ template <int HD> struct PcCfg {
   static constexpr int OFF_RING = 2 * TILE;
   static constexpr int OFF_BARS = OFF_RING + SLOTS * TILE;
   static constexpr int OFF_PAIR = OFF_BARS + 256; // a number of each row thread for the row's other one
-  static constexpr int SMEM = OFF_PAIR + 2 * 2 * PC_ROWS * 4;
+  static constexpr int OFF_WORK = OFF_PAIR + 2 * 2 * PC_ROWS * 4;
+  static constexpr int SMEM = OFF_WORK + 64;
   // a CTA's part of a shared pair of tiles, in the tiles' place
   static constexpr int PITCH = HD + 4; // floats of a row: neighbours' 16-byte pieces fall into different banks
   static constexpr int OFF_ML = 2 * PC_ROWS * PITCH * 4;
@@ -134,16 +135,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-/* 32 scores of a row to probabilities 2^x, x = s * scale - base below 16, packed, and their sum. ALL: none is masked; then some of the pairs
- * are computed on the FMA pipes beside the special function unit, which alone would take as many clocks as a step's products: x = n + f
+/* 32 scores of a row to probabilities 2^x, x = s * scale - base below 16, packed, and their sum. Some of the pairs are computed on the FMA pipes beside the special function unit, which alone would take as many clocks as a step's products: x = n + f
  * with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f by the polynomial of the least greatest relative error with value 1
- * at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent. */
+ * at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent. There what is masked gets 2^-126 and not zero: of no
+ * account beside a row's greatest probability, 2^6 or more. (A row that sees nothing has none: it is zero in the end.) */
 constexpr int PC_GROUP = 8, PC_BY_FMA = 3; // pairs that go step by step together, so many of them on the FMA pipes
-template <typename T, bool ALL>
+template <typename T>
 __device__ __forceinline__ float weights32(const uint32_t *s, float scale, float base, uint32_t *p) {
   constexpr float MAGIC = 12582912.f;
   constexpr bool FOUR = MmaType<T>::bits == 0;
-  constexpr int N = ALL ? PC_BY_FMA : 0;
+  constexpr int N = PC_BY_FMA;
   float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
   for (int g = 0; g < 16; g += PC_GROUP) {
@@ -189,6 +190,9 @@ __device__ __forceinline__ float weights32(const uint32_t *s, float scale, float
   return sum.x + sum.y;
 }
 
+/* a word whose n lowest bits are set */
+__device__ __forceinline__ uint32_t ones_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+
 /* Barriers of a tile's row threads. They come to every one of them whatever became of their bounded waits: whether one ran out is
  * agreed on here too, and then all leave together. */
 __device__ __forceinline__ void rows_sync(int t) {
@@ -209,25 +213,30 @@ template <typename T> constexpr float PC_MOST = MmaType<T>::bits == 0 ? 32768.f 
 /* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. What takes
  * longest comes first, so that it does not begin when the rest is done: in a sequence the last queries, which see most, and among up to
  * 32 sequences those with the longest context. */
-__device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, int lane, int *seq, int *tile) {
-  auto pairs_of = [&](int b) { return b < s.batch ? (seq_rows(s, b).n * G + 2 * PC_ROWS - 1) / (2 * PC_ROWS) : 0; };
+__device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, int lane, int *seq, int *tile, SeqRows *r) {
   if (s.batch <= 32) {
-    const int n = pairs_of(lane), rows = lane < s.batch ? __ldg(s.context + lane) : 0;
+    const int b = min(lane, s.batch - 1), lo = __ldg(s.row_start + b), hi = __ldg(s.row_start + b + 1), rows = __ldg(s.context + b);
+    const SeqRows own = seq_rows(s, lo, hi, rows);
+    const int n = lane < s.batch ? (own.n * G + 2 * PC_ROWS - 1) / (2 * PC_ROWS) : 0;
     int in_front = 0;
-    for (int b = 0; b < s.batch; ++b) {
-      const int nb = __shfl_sync(FULL, n, b), rb = __shfl_sync(FULL, rows, b);
-      in_front += rb > rows || (rb == rows && b < lane) ? nb : 0;
+    for (int k = 0; k < s.batch; ++k) {
+      const int nk = __shfl_sync(FULL, n, k), rk = __shfl_sync(FULL, rows, k);
+      in_front += rk > rows || (rk == rows && k < lane) ? nk : 0;
     }
     const unsigned m = __ballot_sync(FULL, work >= in_front && work < in_front + n);
     if (!m)
       return false;
-    *seq = __ffs(m) - 1;
-    *tile = __shfl_sync(FULL, in_front + n - 1 - work, *seq);
+    const int l = __ffs(m) - 1;
+    *seq = l;
+    *tile = __shfl_sync(FULL, in_front + n - 1 - work, l);
+    r->first = __shfl_sync(FULL, own.first, l);
+    r->n = __shfl_sync(FULL, own.n, l);
+    r->pos = __shfl_sync(FULL, own.pos, l);
     return true;
   }
   int before = 0;
   for (int b0 = 0; b0 < s.batch; b0 += 32) {
-    const int n = pairs_of(b0 + lane);
+    const int n = b0 + lane < s.batch ? (seq_rows(s, b0 + lane).n * G + 2 * PC_ROWS - 1) / (2 * PC_ROWS) : 0;
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -239,6 +248,7 @@ __device__ __forceinline__ bool find_pair(const PagedBatch &s, int G, int work, 
       const int l = __ffs(m) - 1;
       *seq = b0 + l;
       *tile = __shfl_sync(FULL, before + upto - 1 - work, l);
+      *r = seq_rows(s, *seq);
       return true;
     }
     before += __shfl_sync(FULL, upto, 31);
@@ -269,6 +279,10 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Cfg::OFF_BARS + 224);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Cfg::OFF_BARS + 232);
 
+  if (tid == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)));
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)));
+  }
   if (tid == 0) {
     for (int i = 0; i < Cfg::SLOTS; ++i) {
       mbar_init(FULL_BAR(i), 1);
@@ -298,14 +312,30 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   pdl_wait();
 
   const int parts = cluster_size(), part = cluster_rank(), G = g.hq / g.hkv, item = blockIdx.x / parts, h = item % g.hkv;
-  int seq = 0, tile = 0;
-  const bool any = find_pair(s, G, item / g.hkv, lane, &seq, &tile); // the same in every CTA of a cluster
-  SeqRows r = {};
-  if (any)
-    r = seq_rows(s, seq);
-  const int flat0 = tile * 2 * PC_ROWS, rows = any ? min(2 * PC_ROWS, r.n * G - flat0) : 0;
+  // What the CTA works on is found by one warp and stays in shared memory: held in registers meanwhile it costs the row threads spills
+  volatile int *work = reinterpret_cast<volatile int *>(smem + Cfg::OFF_WORK); // rows, sequence, first row of q, position, place in the group
+  if (warp == 0) {
+    int seq = 0, tile = 0;
+    SeqRows r = {};
+    const bool any = find_pair(s, G, item / g.hkv, lane, &seq, &tile, &r); // the same in every CTA of a cluster
+    const int flat0 = tile * 2 * PC_ROWS, tok0 = flat0 / G;
+    if (lane == 0) {
+      work[0] = any ? min(2 * PC_ROWS, r.n * G - flat0) : 0;
+      work[1] = seq;
+      work[2] = r.first + tok0;
+      work[3] = r.pos + tok0;
+      work[4] = flat0 - tok0 * G;
+    }
+  }
+  __syncthreads();
+  const int rows = work[0], seq = work[1];
   const bool two = rows > PC_ROWS;
-  const Sight sight(r.pos + flat0 / G, any ? r.pos + (flat0 + rows - 1) / G : -1, a.window, a.first, PC_KEYS);
+  // row k of the pair of tiles: its token, counted from the pair's first one, and its head of the group
+  const FastDiv by_g(G);
+  auto token_of = [&](int k) { return by_g.div(work[4] + k); };
+  auto head_of = [&](int k, int token) { return h * G + work[4] + k - token * G; };
+  auto q_row = [&](int token) { return work[2] + token; };
+  const Sight sight(work[3], rows > 0 ? work[3] + token_of(rows - 1) : -1, a.window, a.first, PC_KEYS);
   const int b_lo = (int)((long long)sight.blocks * part / parts), steps = (int)((long long)sight.blocks * (part + 1) / parts) - b_lo;
 
   if (warp >= PC_MMA_WARP)
@@ -313,17 +343,22 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
   if (warp < PC_MMA_WARP) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PC_REGS_ROWS));
     /* ------------------------------ two threads per row ------------------------------ */
-    const int t = warp / PC_ROW_WARPS, half = warp / 4 & 1, wrow = (warp & 3) * 32, row = wrow + lane, flat = flat0 + t * PC_ROWS + row;
-    const bool there = t * PC_ROWS + row < rows;
-    const int p = there ? r.pos + flat / G : -1;
+    const int t = warp / PC_ROW_WARPS, half = warp / 4 & 1, wrow = (warp & 3) * 32, row = wrow + lane, own = t * PC_ROWS + row;
+    const bool there = own < rows, busy = t * PC_ROWS + wrow < rows; // busy: a row of the warp is
+    const int p = there ? work[3] + token_of(own) : -1;
     constexpr int CH = HD / 8; // 16-byte pieces of a row
-#pragma unroll 4
-    for (int i = lane; i < 16 * CH; i += 32) {
-      const int rr = wrow + 16 * half + i / CH, c = i % CH, f = flat0 + t * PC_ROWS + rr;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (t * PC_ROWS + rr < rows && 8 * c < g.hd)
-        w = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (r.first + f / G) * a.ld_q + (size_t)(h * G + f % G) * g.hd + 8 * c);
-      sts128(sbase + t * Cfg::TILE + (c >> 3) * (PC_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), w.x, w.y, w.z, w.w);
+    uint4 w[CH / 2]; // 16 rows of the tile, all on their way together
+#pragma unroll
+    for (int u = 0; u < CH / 2; ++u) {
+      const int i = lane + 32 * u, c = i % CH, k = t * PC_ROWS + wrow + 16 * half + i / CH, tok = token_of(k);
+      w[u] = make_uint4(0, 0, 0, 0);
+      if (k < rows && 8 * c < g.hd)
+        w[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + q_row(tok) * a.ld_q + head_of(k, tok) * g.hd + 8 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < CH / 2; ++u) {
+      const int i = lane + 32 * u, c = i % CH, rr = wrow + 16 * half + i / CH;
+      sts128(sbase + t * Cfg::TILE + (c >> 3) * (PC_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), w[u].x, w[u].y, w[u].z, w[u].w);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -351,28 +386,33 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       fence_after();
       const int j0 = sight.block(b_lo + j) * PC_KEYS;
       const bool all = j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first);
+      if (!all) { // masked where they are: what follows need not know
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          const int k0 = j0 + 64 * half + 32 * c; // bit i: the row sees cache row k0 + i
+          const uint32_t seen = ones_below(p + 1 - k0) & (~ones_below(p + 1 - a.window - k0) | ones_below(a.first - k0));
+          uint32_t sr[32];
+          tmem_ld32(s_at + 32 * c, sr);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            sr[i] = seen >> i & 1 ? sr[i] : 0xff800000u;
+          tmem_st32(s_at + 32 * c, sr);
+        }
+        tmem_wait_st();
+      }
       uint32_t pr[32];
       float sum;
       // A row's probabilities refer to a maximum m that is taken in the first step, and where rows are masked. Other steps go by the m there
       // is; what they give shows whether it does. If not the step begins again, with the maximum.
       for (bool afresh = j == 0 || !all;; afresh = true) {
-        auto scores = [&](int c, uint32_t(&sr)[32]) { // 32 of this half's
-          tmem_ld32(s_at + 32 * c, sr);
-          tmem_wait_ld();
-          if (!all) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int key = j0 + 64 * half + 32 * c + i;
-              if (!(key <= p && (key > p - a.window || key < a.first)))
-                sr[i] = 0xff800000u;
-            }
-          }
-        };
         if (afresh) {
           float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
           for (int c = 0; c < 2; ++c) {
             uint32_t sr[32];
-            scores(c, sr);
+            tmem_ld32(s_at + 32 * c, sr);
+            tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; i += 2)
               mx[i >> 1 & 1] = max3(mx[i >> 1 & 1], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
@@ -405,8 +445,9 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t sr[32];
-          scores(c, sr);
-          sum += all ? weights32<T, true>(sr, a.scale_log2, base, pr + 16 * c) : weights32<T, false>(sr, a.scale_log2, base, pr + 16 * c);
+          tmem_ld32(s_at + 32 * c, sr);
+          tmem_wait_ld();
+          sum += weights32<T>(sr, a.scale_log2, base, pr + 16 * c);
         }
         if (!rows_any(t, !came || (!afresh && sum > PC_MOST<T>)))
           break;
@@ -439,16 +480,17 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       l += *pair_other;
     }
     if (mine && ok) {
-      const int head = h * G + flat % G;
       float inv = 1.f;
       if (parts == 1) {
         float total = l;
-        if (a.sink && m > -INFINITY && there)
-          total += ex2(a.sink[head] * LOG2E - (m - PAGED_LIFT));
-        inv = total == 0.f ? 0.f : 1.f / total;
+        if (a.sink && there)
+          total += ex2(a.sink[head_of(own, token_of(own))] * LOG2E - (m - PAGED_LIFT));
+        inv = m == -INFINITY || total == 0.f ? 0.f : 1.f / total;
       }
-      const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd;
-      float *part_row = reinterpret_cast<float *>(smem) + (t * PC_ROWS + row) * Cfg::PITCH;
+      // Rows by threads would be stored as 16 bytes of 32 rows at a time: they go through shared memory, where the tile's queries were, 16-byte
+      // pieces spread over the banks; fp32 ones directly.
+      const uint32_t turn = sbase + t * Cfg::TILE + row * (HD * 2);
+      float *part_row = reinterpret_cast<float *>(smem) + own * Cfg::PITCH;
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) {
         uint32_t o[32];
@@ -470,20 +512,29 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
           if (parts > 1) {
             *reinterpret_cast<float4 *>(part_row + col) = make_float4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<float4 *>(part_row + col + 4) = make_float4(f[4], f[5], f[6], f[7]);
+          } else if (!a.out_f32) {
+            sts128(turn + ((col >> 3 ^ (row & (HD / 8 - 1))) << 4), pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
           } else if (there && col < g.hd) {
-            if (a.out_f32) {
-              float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + e + col);
-              dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-              dst[1] = make_float4(f[4], f[5], f[6], f[7]);
-            } else {
-              *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + e + col) =
-                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-            }
+            const int token = token_of(own);
+            float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + q_row(token) * a.ld_out + head_of(own, token) * g.hd + col);
+            dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+            dst[1] = make_float4(f[4], f[5], f[6], f[7]);
           }
         }
       }
       if (parts > 1 && half == 0)
-        *reinterpret_cast<float2 *>(smem + Cfg::OFF_ML + 8 * (t * PC_ROWS + row)) = make_float2(m, l);
+        *reinterpret_cast<float2 *>(smem + Cfg::OFF_ML + 8 * own) = make_float2(m, l);
+    }
+    if (mine && parts == 1 && !a.out_f32) {
+      if (!rows_any(t, !ok)) {
+#pragma unroll
+        for (int u = 0; u < CH / 2; ++u) {
+          const int i = lane + 32 * u, c = i % CH, rr = wrow + 16 * half + i / CH, k = t * PC_ROWS + rr, tok = token_of(k);
+          const uint4 v = lds128(sbase + t * Cfg::TILE + rr * (HD * 2) + ((c ^ (rr & (CH - 1))) << 4));
+          if (k < rows && 8 * c < g.hd)
+            *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + q_row(tok) * a.ld_out + head_of(k, tok) * g.hd + 8 * c) = v;
+        }
+      }
     }
   } else if (warp < PC_COPY_WARP) {
     /* ------------------------------ products ------------------------------ */
@@ -589,7 +640,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
     const uint32_t raised = neighbour_raised(smem_u32(const_cast<int *>(abort_flag)), lane);
     if (warp < PC_MMA_WARP && !__any_sync(FULL, raised)) {
       for (int R = part + parts * warp; R < rows; R += parts * PC_MMA_WARP) {
-        const int flat = flat0 + R, head = h * G + flat % G, col = 4 * lane;
+        const int tok = token_of(R), head = head_of(R, tok), col = 4 * lane;
         float2 ml[8];
         float4 v[8];
 #pragma unroll
@@ -619,7 +670,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         if (a.sink && big > -INFINITY)
           total += ex2(a.sink[head] * LOG2E - (big - PAGED_LIFT));
         const float inv = total == 0.f ? 0.f : 1.f / total;
-        const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd + col;
+        const long long e = q_row(tok) * a.ld_out + (long long)head * g.hd + col;
         if (col < g.hd) {
           if (a.out_f32)
             *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + e) = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);

@@ -33,7 +33,7 @@ int check_paged(const char *what, const nntr_paged_cache *c, const nntr_paged_ba
     return set_error(NNTR_CUDA_ERR_INVALID, "%s: null pointer", what);
   if (c->dtype != NNTR_F16 && c->dtype != NNTR_BF16)
     return set_error(NNTR_CUDA_ERR_UNSUPPORTED, "%s: caches of fp16 or bf16 (dtype %d)", what, c->dtype);
-  if (!c->n_heads_q || !c->n_heads_kv || c->n_heads_q % c->n_heads_kv || c->n_heads_q > 65535)
+  if (!c->n_heads_q || !c->n_heads_kv || c->n_heads_q % c->n_heads_kv || c->n_heads_q > 4096)
     return set_error(NNTR_CUDA_ERR_INVALID, "%s: %u query heads on %u kv heads", what, c->n_heads_q, c->n_heads_kv);
   if (c->head_dim == 0 || c->head_dim % 8)
     return set_error(NNTR_CUDA_ERR_INVALID, "%s: need head_dim %% 8 == 0 (head_dim=%u)", what, c->head_dim);
@@ -47,7 +47,7 @@ int check_paged(const char *what, const nntr_paged_cache *c, const nntr_paged_ba
                      (long long)stride, (long long)dense);
   if (c->n_pages == 0 || c->n_pages > 0x7fffffffu)
     return set_error(NNTR_CUDA_ERR_INVALID, "%s: a pool of %u pages", what, c->n_pages);
-  if (b->batch > 65535 || b->tokens > 0x7fffffffu / 1024 || b->max_new > b->tokens)
+  if (b->batch > 65535 || b->tokens > 0x40000000u / c->n_heads_q || b->max_new > b->tokens)
     return set_error(NNTR_CUDA_ERR_INVALID, "%s: batch of %u sequences, %u rows, %u of them of one sequence", what, b->batch, b->tokens,
                      b->max_new);
   if (b->ld_table > 0x7fffffffu / c->page_size)

@@ -488,9 +488,13 @@ int launch_paged_attention(const nntr_paged_cache *c, const nntr_paged_batch *b,
   constexpr int NONE = 0x3fffffff;
   AttendArgs a = {q, c->kcache, c->vcache, out, sink, ld_q, ld_out, (int)std::min(window, (unsigned)NONE),
                   (int)std::min(first_tokens, (unsigned)NONE), out_dtype == NNTR_F32, LOG2E / sqrtf((float)g.hd)};
-  if (s.max_new * (g.hq / g.hkv) > 16)
+  // Up to 32 rows of a kv head's group take the kernel above: its tiles of 16 read the cache twice, the second time from L2, but the other one's
+  // steps of 128 rows cost the same for one query row as for 128 (4 x 8000 rows of cache, 8 kv heads of 128: 20 query rows 31.5 and 40.5
+  // us, 36 rows 56 and 41). Up to 64 where few CTAs are busy anyway (1 x 8000: 64 rows 19.4 and 23.8; 128 rows 30.5 and 25.2).
+  const long long rows = (long long)s.max_new * (g.hq / g.hkv);
+  const int tiles = (int)((rows + 15) / 16);
+  if (rows > 32 && (rows > 64 || (long long)tiles * g.hkv * s.batch > sm_count() / 4))
     return launch_paged_attention_chunk(a, c->dtype, g, s, b->max_rows, flags, st);
-  const int G = g.hq / g.hkv, tiles = (int)(((long long)s.max_new * G + 15) / 16);
   if (c->dtype == NNTR_F16)
     return g.hd <= 64 ? launch_few<__half, 64, 4>(a, g, s, b->max_rows, tiles, flags, st) : launch_few<__half, 128, 4>(a, g, s, b->max_rows, tiles, flags, st);
   return g.hd <= 64 ? launch_few<__nv_bfloat16, 64, 4>(a, g, s, b->max_rows, tiles, flags, st)

@@ -614,8 +614,8 @@ def _paged(torch, kcache, vcache, n_heads_q: int, page_table, row_start, context
     if len(shape) != 4 or vcache.shape != shape or vcache.dtype is not t or vcache.stride() != stride:
         raise ValueError("kcache and vcache: [n_pages, page_size, n_heads_kv, head_dim], alike in type and strides")
     pages, ps, hkv, hd = shape
-    if stride[3] != 1 or stride[2] != hd or stride[1] != hkv * hd:
-        raise ValueError("kcache and vcache: the rows of a page lie back to back")
+    if stride[3] != 1 or stride[2] != hd or stride[1] != hkv * hd or (pages > 1 and stride[0] < ps * hkv * hd):
+        raise ValueError("kcache and vcache: the rows of a page lie back to back, pages do not overlap")
     if t is torch.float16:
         dtype = capi.F16
     elif t is torch.bfloat16:

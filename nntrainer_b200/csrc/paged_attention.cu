@@ -273,9 +273,9 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
         }
     uint32_t pf[4];
     float sum[2];
-    // A row's probabilities refer to a maximum m that is taken in the first block, and where rows are masked. Other blocks go by the m there
-    // is; what they give shows whether it does. If not they begin again, with the maximum.
-    for (bool afresh = i == 0 || !whole;; afresh = true) {
+    // A row's probabilities refer to a maximum m that is taken in the first block that it sees something of, and where rows are masked. Other
+    // blocks go by the m there is; what they give shows whether it does. If not they begin again, with the maximum.
+    for (bool afresh = !whole || __any_sync(FULL, m[0] == -INFINITY || m[1] == -INFINITY);; afresh = true) {
       if (afresh) {
         float mx[2], keep[2];
 #pragma unroll

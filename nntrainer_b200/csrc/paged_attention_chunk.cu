@@ -381,6 +381,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
           if (item + Cfg::SLOTS < 2 * steps) // nobody waits for a slot that is not filled again
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(EMPTY_BAR(item % Cfg::SLOTS)), "r"(two ? 1 : 2) : "memory");
     };
+    bool unset = true; // a row of the tile has no maximum yet
     for (int j = 0; mine && j < steps; ++j) {
       const bool came = pc_wait(S_BAR(t), j & 1, abort_flag);
       fence_after();
@@ -403,9 +404,9 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       }
       uint32_t pr[32];
       float sum;
-      // A row's probabilities refer to a maximum m that is taken in the first step, and where rows are masked. Other steps go by the m there
-      // is; what they give shows whether it does. If not the step begins again, with the maximum.
-      for (bool afresh = j == 0 || !all;; afresh = true) {
+      // A row's probabilities refer to a maximum m that is taken in the first step that it sees something of, and where rows are masked. Other
+      // steps go by the m there is; what they give shows whether it does. If not the step begins again, with the maximum.
+      for (bool afresh = unset || !all;; afresh = true) {
         if (afresh) {
           float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
@@ -439,6 +440,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
               }
             }
           }
+          unset = rows_any(t, m == -INFINITY);
         }
         const float base = m == -INFINITY ? 0.f : m - PAGED_LIFT;
         sum = 0.f;

@@ -50,8 +50,8 @@ int check_paged(const char *what, const nntr_paged_cache *c, const nntr_paged_ba
   if (b->batch > 65535 || b->tokens > 0x40000000u / c->n_heads_q || b->max_new > b->tokens)
     return set_error(NNTR_CUDA_ERR_INVALID, "%s: batch of %u sequences, %u rows, %u of them of one sequence", what, b->batch, b->tokens,
                      b->max_new);
-  if (b->ld_table > 0x7fffffffu / c->page_size)
-    return set_error(NNTR_CUDA_ERR_INVALID, "%s: a page table of %u entries per sequence", what, b->ld_table);
+  if (b->ld_table > 0x20000000u / c->page_size) // positions and differences of them stay in 32 bits
+    return set_error(NNTR_CUDA_ERR_INVALID, "%s: a page table of %u entries per sequence; contexts of at most 2^29 rows", what, b->ld_table);
   if (b->batch && (!b->row_start || !b->context || (b->ld_table && !b->page_table)))
     return set_error(NNTR_CUDA_ERR_INVALID, "%s: null pointer", what);
   int shift = 0;

@@ -141,6 +141,16 @@ def test_windows_first_tokens_and_sinks(be, heads, new, ctx, window, first, with
     c.check(c.attend(be, **kw), **kw)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,ctx,window", [(2, 2001, 513), (2, 2001, 512), (3, 2001, 514), (100, 2000, 494), (100, 2000, 493), (100, 2000, 495),
+                                            (40, 700, 60), (300, 1000, 129)])
+def test_the_first_rows_read_are_out_of_sight_for_some(be, dtype, new, ctx, window):
+    """The window of a tile's first query begins at the end of a block that its later ones do not see at all."""
+    for heads in ((16, 2, 96), (4, 4, 64)):
+        c = Case([new, 1], [ctx, 5], heads, dtype, 32, seed=33)
+        c.check(c.attend(be, window=window), window=window)
+
+
 @pytest.mark.parametrize("new", [1, 65])
 def test_what_no_query_sees_may_be_anything(be, new):
     """NaN and infinities in rows that have left the window, in the rest of the last page and in pages of others."""
@@ -171,6 +181,16 @@ def test_results_in_fp32_strided_operands_rows_behind(be, new, ctx):
     assert c.attend(be, q=q, out=view) is view
     c.check(view)
     assert bool((out[:, :8] == 7).all()) and bool((out[:, -8:] == 7).all()) and bool((out[c.starts[-1]:] == 7).all())
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 128), (8, 1, 64), (3, 1, 96)])
+@pytest.mark.parametrize("batch,most", [(150, 1), (129, 3), (70, 5), (33, 90), (40, 16), (3, 16), (2, 8)])
+def test_many_sequences_and_few_rows(be, heads, batch, most):
+    new = [1 + (7 * b) % most for b in range(batch)]
+    ctx = [n + (37 * b) % 211 for b, n in enumerate(new)]
+    c = Case(new, ctx, heads, BF16 if batch % 2 else F16, 16, seed=batch)
+    c.check(c.attend(be))
+    c.check(c.attend(be, window=50, first_tokens=3), window=50, first_tokens=3)
 
 
 @pytest.mark.parametrize("new", [1, 150])

@@ -677,10 +677,10 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
         atomicAdd(&sh.sub[sh.i[i] / a.sub_len], sh.w[i]);
     __syncthreads();
   };
-  /* Where few tokens, no more than SP_FEW, lie above the cut and pass min_p (value `passes`): each is compared with each. all: the sum that top_p refers to (with top_k it
-   * is that of the tokens top_k leaves). False: there are more. */
-  auto among_few = [&](uint32_t passes, unsigned long long all) {
-    const uint32_t least = has_k && has_p ? cut : max(cut, passes); // that sum has the tokens too that min_p drops
+  /* Where few tokens, no more than SP_FEW, lie above the cut and pass min_p (value `passes`): each is compared with each. all: the sum that
+   * top_p refers to, if it is known; else it is that of the tokens top_k leaves, which all lie above the cut then. False: there are more. */
+  auto among_few = [&](uint32_t passes, unsigned long long all, bool known) {
+    const uint32_t least = has_p && !known ? cut : max(cut, passes); // that sum has the tokens too that min_p drops
     if (tid == 0)
       sh.few = 0;
     __syncthreads();
@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
       }
       bool mine = there && (!has_k || rank < top_k);
       if (has_p) {
-        if (has_k)
+        if (!known)
           all = warp_sum(mine ? w : 0);
         mine = mine && in_front < (unsigned long long)ceil(top_p * (double)all);
       }
@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
       }
     bool mine = there && (!has_k || rank < top_k);
     if (has_p) {
-      if (has_k)
+      if (!known)
         all = cta_sum(sh, mine ? w : 0);
       mine = mine && in_front < (unsigned long long)ceil(top_p * (double)all);
     }
@@ -801,11 +801,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     const bool early = open && least > 1u && !deep_k; // whatever top_p says, the kept tokens are listed
     if (early)
       say(0);
-    if (enough && (!has_p || has_k || least > 1u || all_listed) && among_few(least, sum))
+    if (enough && (!has_p || has_k || least > 1u || all_listed) && among_few(least, sum, !has_k))
       return;
     if (has_k && top_k < listed) {
       cut_by_count(head, top_k);
-      if (among_few(least, sum))
+      if (among_few(least, sum, !has_k))
         return;
     }
     if (has_p && enough) {
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     if (open && !early)
       say(word);
     if (word == 0) {
-      if (of_cut && among_few(least, sum))
+      if (of_cut && among_few(least, sum, true))
         return;
       place_cut();
       const unsigned long long total = list_sum(kept);

@@ -70,11 +70,11 @@ def check(be, x, u, **kw):
 
 FILTERS = [dict(), dict(t=0.7), dict(k=1), dict(k=5), dict(k=50, t=1.3), dict(k=2000), dict(p=0.9), dict(p=0.5, t=0.6), dict(p=1e-6), dict(p=0.9999),
            dict(m=0.05), dict(m=1.0), dict(k=40, p=0.95), dict(k=40, p=0.8, m=0.1, t=0.8), dict(t=0.0), dict(p=0.0), dict(t=5.0, p=0.97), dict(t=0.05),
-           dict(k=20000), dict(k=20000, p=0.9), dict(p=0.99, m=1e-4), dict(m=1e-6), dict(t=1e-20), dict(t=1e20)]
+           dict(k=20000), dict(k=20000, p=0.9), dict(k=500, p=0.5, t=0.8), dict(k=200, p=0.7, m=1e-3), dict(k=900, p=0.99), dict(p=0.99, m=1e-4), dict(m=1e-6), dict(t=1e-20), dict(t=1e20)]
 
 
 @pytest.mark.parametrize("kw", FILTERS)
-@pytest.mark.parametrize("rows,n", [(1, 1), (3, 2), (2, 31), (4, 257), (3, 1000), (2, 32000), (5, 50257), (2, 151936)])
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 2), (2, 31), (4, 257), (3, 1000), (3, 6144), (4, 9000), (2, 32000), (5, 50257), (2, 151936)])
 def test_against_the_definition(be, rows, n, kw):
     g = torch.Generator(device="cuda").manual_seed(rows * n)
     x = 2 * torch.randn(rows, n, generator=g, device="cuda")

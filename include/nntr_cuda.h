@@ -347,7 +347,7 @@ int nntr_cuda_attention_rows_dev(const nntr_attn_desc *a, unsigned pos, unsigned
 /** One layer's key/value cache in pages, which many sequences share: page p of either cache begins p * page_stride elements behind
  *  its pointer and holds page_size rows of [kv head][head_dim], as a row of the contiguous caches above. Device pointers,
  *  16-byte aligned; page_stride 0 = pages back to back, else a multiple of 8. dtype NNTR_F16 or NNTR_BF16; page_size 16, 32, 64, 128 or
- *  256; head_dim a multiple of 8 of at most 128; n_heads_q a multiple of n_heads_kv. */
+ *  256; head_dim a multiple of 8 of at most 128; n_heads_q a multiple of n_heads_kv, at most 4096. */
 typedef struct {
   unsigned n_heads_q, n_heads_kv, head_dim;
   int dtype;
@@ -360,7 +360,8 @@ typedef struct {
  *  in page page_table[b * ld_table + r / page_size], which other sequences may share. The arrays are device memory, so that a
  *  captured graph can be replayed with other contents; the numbers beside them are host-side bounds: `tokens` rows that q and the
  *  results hold, no more than max_new rows of one sequence, contexts of about max_rows (0: not known; it chooses how the work is split,
- *  any context is right). Rows of q and of the results behind the last sequence are neither read nor written.
+ *  any context is right). Rows of the results behind the last sequence are left as they are. At most 65535 sequences, 2^30 / n_heads_q
+ *  rows and ld_table * page_size = 2^29.
  *  Arrays that contradict the bounds or themselves (more rows than max_new, a context of fewer rows than the sequence has new ones,
  *  rows behind the page table, a page outside the pool that is needed) touch no memory out of range: rows of such a page read as zeros
  *  and are not stored, queries in front of position 0 see nothing, rows beyond the bounds are left as they were, and
@@ -406,8 +407,10 @@ int nntr_cuda_copy_pages_dev(void *base, unsigned arrays, int64_t array_bytes, i
  *  row_params: device [rows][4] of (temperature, top_k, top_p, min_p) for each row in place of the four numbers, or NULL; there a
  *  temperature or top_p that is not above 0 means the greatest logit.
  *  idx_out (uint32) and / or idx_out_f (as a float) may be NULL; prob_out, or NULL: the token's weight over the kept ones' sum.
- *  Weights are double precision, sums are exact: the token does not depend on how the work is split. Up to 2^20 logits,
- *  65535 rows. */
+ *  temperature: at most 1e30. The greatest weights (from 2^-14 of the greatest one on, a few thousand of them) are double precision, the
+ *  others fp32 to 2^-22; sums are exact in whole multiples of 2^-44 of the greatest weight: the token does not depend on how the work is
+ *  split, and a draw is another than exact arithmetic's only where u or a threshold falls within about 2^-21 of a border. Up to 2^20
+ *  logits, 65535 rows. */
 int nntr_cuda_sample_dev(const float *logits, int64_t rows, int64_t n, int64_t ld, const float *u, double temperature, unsigned top_k,
                          double top_p, double min_p, const float *row_params, unsigned *idx_out, float *idx_out_f, float *prob_out,
                          unsigned flags, void *stream);

@@ -698,7 +698,7 @@ def paged_attention(q, kcache, vcache, page_table, row_start, context, max_new: 
             raise ValueError("out: [tokens, n_heads_q, head_dim] in the caches' type or fp32")
         dtype = capi.F32 if out.dtype is torch.float32 else dtype
     rc = lib().nntr_cuda_paged_attention_dev(
-        c, b, q.data_ptr(), ld[0], 0xFFFFFFFF if window is None else window, first_tokens,
+        c, b, q.data_ptr(), ld[0], 0xFFFFFFFF if window is None else min(window, 0xFFFFFFFF), min(first_tokens, 0xFFFFFFFF),
         None if sink is None else _typed(sink, "sink", torch.float32, hq),
         out.data_ptr(), dtype, ld_out, capi.GEMV_PDL if pdl else 0, _stream())
     if rc:
@@ -756,7 +756,7 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     else:
         _typed(prob, "out", f32, rows)
     rc = lib().nntr_cuda_sample_dev(
-        logits.data_ptr(), rows, n, stride[0] if len(shape) == 2 else n, u.data_ptr(), temperature, top_k, top_p, min_p,
+        logits.data_ptr(), rows, n, stride[0] if len(shape) == 2 else n, u.data_ptr(), temperature, min(top_k, n), top_p, min_p,
         None if params is None else _typed(params, "params", f32, 4 * rows), idx.data_ptr(), idx_f.data_ptr(), prob.data_ptr(),
         capi.GEMV_PDL if pdl else 0, _stream())
     if rc:
@@ -805,8 +805,8 @@ class PagedCache:
 
     def _copy(self, src: list, dst: list) -> None:
         torch = _torch()
-        if src:
-            both = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
+        for i in range(0, len(src), 65535):  # as many as a launch takes
+            both = torch.tensor([src[i:i + 65535], dst[i:i + 65535]], dtype=torch.int32).to(self.device)
             copy_pages(self.kv, both[0], both[1])
 
     def new(self) -> int:

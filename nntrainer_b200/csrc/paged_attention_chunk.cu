@@ -5,18 +5,23 @@
  *
  * The formulas are those of paged_attention.cu. A tile is 128 rows of (token, query head of one kv head's group); a CTA holds two of
  * them against the same cache rows, in steps of 128:
- *   warps 0-7, 8-15 two threads per row of the first / second tile, one half of the step's rows each: S from tensor memory, running maximum, probabilities back to tensor
- *                   memory over S as the next product's 16-bit operand, their sum. O is multiplied in place only when a row's maximum has grown by
- *                   more than 2^7 since it was last done: until then the probabilities are that much larger, which their 16-bit type holds
- *                   (fp16: 2^8 to keep small ones out of the subnormal numbers, times 2^7).
+ *   warps 0-7, 8-15 two threads per row of the first / second tile, one half of the step's rows each: S from tensor memory, probabilities
+ *                   back over it as the next product's 16-bit operand, their sum. O is multiplied in place only where a row's probabilities
+ *                   would outgrow their type with the maximum that they refer to.
  *   warps 16, 17    one for each tile; a thread issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as
- *                   it lies, dimensions contiguous; the first 64 rows as soon as their probabilities are there). While one tile's
- *                   probabilities are computed the other tile's products run.
+ *                   it lies, dimensions contiguous). While one tile's probabilities are computed the other tile's products run.
  *   warp 18         TMA copies of K and V tiles through one ring of slots: a box per page (128 rows of it at most) and 64 dimensions.
- * Tensor memory: S (P) 128 columns a tile, O head_dim columns a tile. A step's products take 4 * 128 * 128 * head_dim flop a tile, its 16384
- * exponentials as many clocks (16 a clock and SM) as its products at head_dim 128.
+ * Tensor memory: S (P) 128 columns a tile, O head_dim columns a tile.
  * Few tiles: the CTAs of a cluster share a pair of tiles along the cache rows and join through each other's shared memory.
  * Every wait is bounded (pipeline.cuh).
+ *
+ * What bounds it. A step's products take 2 * 1024 clocks at head_dim 128, its 2 * 16384 exponentials as many on the special function unit
+ * alone (16 a clock). A tile goes round in about 2800: 1400 from its scores to its probabilities (900 of them exponentials of two warps
+ * per scheduler), 1030 its products, the rest hand-overs; two tiles overlap. 2 x 2048 tokens of 32 heads of 128 on 8 kv heads at up
+ * to 16384 rows: 852 us, 1033 TFLOP/s, at the power limit when it runs for long (1.67 GHz, 990 W). On the way there: 1185
+ * with all exponentials on the special function unit, a maximum in every step and both tiles' products issued by one thread; 1024 with
+ * exponentials on two units; 960 with the products in turn (TURN_BAR), operands in uniform registers and maxima where a sum asks for them;
+ * 890 with two threads per row (a warp alone on its scheduler waits for its own instructions); the masks out of the step's way 852.
  */
 #include "cluster.cuh"
 #include "paged_attention.cuh"
@@ -387,7 +392,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       fence_after();
       const int j0 = sight.block(b_lo + j) * PC_KEYS;
       const bool all = j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first);
-      if (!all) { // masked where they are: what follows need not know
+      if (!all && busy) { // masked where they are: what follows need not know
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           const int k0 = j0 + 64 * half + 32 * c; // bit i: the row sees cache row k0 + i
@@ -410,7 +415,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         if (afresh) {
           float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < (busy ? 2 : 0); ++c) {
             uint32_t sr[32];
             tmem_ld32(s_at + 32 * c, sr);
             tmem_wait_ld();
@@ -440,17 +445,18 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
               }
             }
           }
-          unset = rows_any(t, m == -INFINITY);
+          unset = rows_any(t, there && m == -INFINITY);
         }
         const float base = m == -INFINITY ? 0.f : m - PAGED_LIFT;
         sum = 0.f;
+        if (busy)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t sr[32];
-          tmem_ld32(s_at + 32 * c, sr);
-          tmem_wait_ld();
-          sum += weights32<T>(sr, a.scale_log2, base, pr + 16 * c);
-        }
+          for (int c = 0; c < 2; ++c) {
+            uint32_t sr[32];
+            tmem_ld32(s_at + 32 * c, sr);
+            tmem_wait_ld();
+            sum += weights32<T>(sr, a.scale_log2, base, pr + 16 * c);
+          }
         if (!rows_any(t, !came || (!afresh && sum > PC_MOST<T>)))
           break;
         if (rows_any(t, !came)) {
@@ -460,9 +466,11 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       }
       if (!ok)
         break;
-      tmem_st32(s_at, pr);
-      l += sum;
-      tmem_wait_st();
+      if (busy) { // else: nobody asks for what comes of those rows
+        tmem_st32(s_at, pr);
+        l += sum;
+        tmem_wait_st();
+      }
       fence_before();
       __syncwarp();
       if (lane == 0)

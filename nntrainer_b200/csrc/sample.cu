@@ -16,6 +16,10 @@
  * the cuts and the draw by digits of eight bits, each a histogram. Where a cut lies below the list, the histogram says
  * about where; one more pass lists the logits around it and sums what is above, slice by slice. Where that does not do either (very many
  * equal logits, top_k and top_p both far down) the whole cluster goes by digits over the whole row.
+ *
+ * What bounds it: for a row the chain of passes (greatest logit, histogram, list, cuts, draw: five to eight barriers of the cluster or CTA
+ * each), one row of 151936 logits 13.9 us; for many rows the instructions that a logit takes in the passes, 128 rows of 201088 (103 MB) 69 us,
+ * 1.5 TB/s. All weights in double precision and digits over the whole row: 1240 and 2234 us.
  */
 #include "cluster.cuh"
 #include "pipeline.cuh"

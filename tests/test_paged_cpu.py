@@ -214,3 +214,16 @@ def test_compact_moves_used_pages_to_the_front():
     assert c.compact() == 0
     c.reserve([b], [16])
     assert c.pages(b)[-1] == len(used)
+
+
+def test_more_copies_than_a_launch_takes(monkeypatch):
+    calls = []
+    monkeypatch.setattr(be, "copy_pages", lambda kv, src, dst: calls.append((src.tolist(), dst.tolist())))
+    c = be.PagedCache(1, 4, 16, 1, 8, device="cpu")
+    n = 2 * 65535 + 3
+    c._copy(list(range(n)), list(range(n, 2 * n)))
+    assert [len(s) for s, _ in calls] == [65535, 65535, 3]
+    assert sum((s for s, _ in calls), []) == list(range(n)) and sum((d for _, d in calls), []) == list(range(n, 2 * n))
+    calls.clear()
+    c._copy([], [])
+    assert not calls

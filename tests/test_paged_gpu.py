@@ -224,6 +224,14 @@ def test_a_pool_beyond_two_gigaelements(be, new):
     c.check(c.attend(be))
 
 
+@pytest.mark.parametrize("new", [[1, 2], [70, 3]])
+def test_counts_beyond_32_bits(be, new):
+    c = Case(new, [100, 300], (8, 2, 64), seed=31)
+    want = c.attend(be)
+    assert torch.equal(c.attend(be, window=2 ** 32 + 5), want)
+    assert torch.equal(c.attend(be, window=5, first_tokens=2 ** 32 + 5), want)
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_captured_and_replayed_with_other_contents(be, new):
     c = Case([new, new], [300, 200], (8, 2, 128), F16, 16, seed=8)

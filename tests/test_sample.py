@@ -148,6 +148,14 @@ def test_strided_rows_and_given_results(be):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_counts_beyond_32_bits_and_the_least_temperature(be):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(5, 9000, generator=g, device="cuda")
+    u = torch.rand(5, generator=g, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(be.sample(x, u, top_k=2 ** 32 + 1), be.sample(x, u)))
+    assert torch.equal(be.sample(x, u, temperature=5e-324, top_p=0.9)[0].long(), x.argmax(1))
+
+
 def test_greedy_is_the_argmax(be):
     g = torch.Generator(device="cuda").manual_seed(8)
     x = torch.randint(0, 50, (30, 7000), generator=g, device="cuda").float()

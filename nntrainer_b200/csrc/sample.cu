@@ -18,8 +18,8 @@
  * equal logits, top_k and top_p both far down) the whole cluster goes by digits over the whole row.
  *
  * What bounds it: for a row the chain of passes (greatest logit, histogram, list, cuts, draw: five to eight barriers of the cluster or CTA
- * each), one row of 151936 logits 13.9 us; for many rows the instructions that a logit takes in the passes, 128 rows of 201088 (103 MB) 69 us,
- * 1.5 TB/s. All weights in double precision and digits over the whole row: 1240 and 2234 us.
+ * each), one row of 151936 logits 13.9 us; for many rows the FMA pipes in the second reading (17 operations a logit), 128 rows of 201088 (103 MB) 54 us,
+ * 1.9 TB/s. All weights in double precision and digits over the whole row: 1240 and 2234 us.
  */
 #include "cluster.cuh"
 #include "pipeline.cuh"
@@ -40,6 +40,7 @@ constexpr int SP_FEW = 128;                // tokens that are compared each with
 constexpr int SP_BINS = 512;               // of the estimate, over 46 powers of two of the weight
 constexpr int SP_EVERY = 8;                // every eighth block of 128 logits is in it
 constexpr double SP_ONE = 17592186044416.0; // 2^44: 2^20 logits of the greatest weight stay in 64 bits
+constexpr float SP_HIGH = 6.f, SP_LOW = 1.5f / 2097152.f; // the last bit of the one plus a weight is 2^-21, of the other plus up to 2^-22 either way 2^-44
 constexpr double SP_EXACT_NATS = 9.7;      // (x - max) / T of the lightest token in double precision: 2^-14
 constexpr unsigned SP_MAX_N = 1u << 20;
 
@@ -76,7 +77,7 @@ __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_flo
 
 /* Weights of a row. 2^f on [-1/2, 1/2]: polynomial of the least greatest relative error (2^-28.9) with value 1 at 0. */
 struct Weigher {
-  float mx, exact_from; // the greatest logit; from here up in double precision
+  float mx, exact_from, least; // the greatest logit; from here up in double precision; logits further down weigh as little as this one, nothing
   bool fp32;            // others in fp32; else all in double precision
   double top, per_t;
   float c_hi, c_lo, m_hi, m_lo; // log2(e) / T, and times the greatest logit, each as a sum of two
@@ -89,16 +90,21 @@ struct Weigher {
     m_hi = (float)(rint(m * 8.0) * 0.125); // plus a small whole number it is exact
     m_lo = (float)(m - (double)m_hi);
     fp32 = fabs(m) < 1048576.0;
+    least = (float)(top - 60.0 / c);
     if (!fp32) { // it is not: few logits are that large against the temperature
-      c_hi = c_lo = m_hi = m_lo = 0.f;
+      c_hi = c_lo = m_lo = least = 0.f; // what is in no order weighs 2^-60
+      m_hi = 60.f;
       exact_from = -3.402823466e38f;
     }
   }
   __device__ __forceinline__ double exactly(float x) const { return x == mx ? 1.0 : x > -INFINITY ? exp(((double)x - top) * per_t) : 0.0; }
   __device__ __forceinline__ unsigned long long exact_one(float x) const { return __double2ull_rn(exactly(x) * SP_ONE); }
-  /* two logits, sums of their weights' integers; two operations in one instruction where they are fp32 */
-  __device__ __forceinline__ void in_fp32(float x0, float x1, unsigned long long *w0, unsigned long long *w1) const {
+  /* Two logits, their weights rounded to whole multiples of 2^-44: of 2^-21 in the low bits of w + 6, what is left of that, of 2^-44 in those
+   * of the rest + 1.5 * 2^-21. So most of it is fp32, two operations in one instruction, and sums of weights are sums of words. (64-bit shifts,
+   * comparisons and selections run at half the rate: with them the reading of 128 rows took 1.6 times as long.) */
+  __device__ __forceinline__ void in_fp32(float x0, float x1, uint32_t (&hi)[2], uint32_t (&lo)[2]) const {
     constexpr float MAGIC = 12582912.f; // 1.5 * 2^23: the sum's low bits are the nearest whole number
+    x0 = fmaxf(x0, least), x1 = fmaxf(x1, least); // NaN is `least` too
     float y0 = -m_hi, y1 = -m_hi, g0 = -m_lo, g1 = -m_lo;
     fma2(y0, y1, x0, x1, c_hi, c_hi);
     fma2(g0, g1, x0, x1, c_lo, c_lo);
@@ -118,19 +124,21 @@ struct Weigher {
     fma2(q0, q1, r0, r1, f.x, f.y);
     r0 = r1 = 1.f;
     fma2(r0, r1, q0, q1, f.x, f.y);
-    *w0 = y0 > -46.f ? fixed_of(r0, t.x) : 0ull;
-    *w1 = y1 > -46.f ? fixed_of(r1, t.y) : 0ull;
+    const float w0 = __uint_as_float(__float_as_uint(r0) + (__float_as_uint(t.x) << 23)), w1 = __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t.y) << 23));
+    const float2 a = add2(w0, w1, SP_HIGH, SP_HIGH), h = add2(a.x, a.y, -SP_HIGH, -SP_HIGH), l = add2(w0, w1, -h.x, -h.y), b = add2(l.x, l.y, SP_LOW, SP_LOW);
+    hi[0] = __float_as_uint(a.x), hi[1] = __float_as_uint(a.y);
+    lo[0] = __float_as_uint(b.x), lo[1] = __float_as_uint(b.y);
   }
-  static __device__ __forceinline__ unsigned long long fixed_of(float r, float t) { // r * 2^n * 2^44, n in t's low bits
-    const uint32_t b = __float_as_uint(r) + (__float_as_uint(t) << 23);
-    return (unsigned long long)((b & 0x7fffff) | 0x800000) << 21 >> (127 - (b >> 23));
+  /* a sum of n weights from the sums of their words, for up to 128 of them */
+  static __device__ __forceinline__ unsigned long long sum_of(uint32_t hi, uint32_t lo, int n) {
+    return ((long long)(int)(hi - n * __float_as_uint(SP_HIGH)) << 23) + (int)(lo - n * __float_as_uint(SP_LOW));
   }
   __device__ __forceinline__ unsigned long long operator()(float x) const {
     if (x >= exact_from)
       return exact_one(x);
-    unsigned long long w, same;
-    in_fp32(x, x, &w, &same);
-    return w;
+    uint32_t hi[2], lo[2];
+    in_fp32(x, x, hi, lo);
+    return sum_of(hi[0], lo[0], 1);
   }
   /* the least logit with a weight of at least w, but no greater than the greatest */
   __device__ float least_with(double w) const {
@@ -296,7 +304,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
   // this warp's slice of the row: the CTAs take slices in turn, so that none has all of the tokens that a model likes (low indices, often)
   const unsigned sub = warp * parts + part, s0 = min(a.n, sub * a.sub_len), s1 = min(a.n, s0 + a.sub_len);
   constexpr int AT = 4; // loads of a lane on their way at a time
-  auto for_slice = [&](auto f) { // f(index, four logits); what is behind the slice is NaN
+  auto for_slice = [&](auto f, auto after) { // f(index, four logits); what is behind the slice is NaN; after() comes after AT of them
     for (unsigned i0 = s0 + 4 * lane; i0 - 4 * lane < s1; i0 += 128 * AT) {
       float v[AT][4];
 #pragma unroll
@@ -314,12 +322,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
 #pragma unroll
       for (int k = 0; k < AT; ++k)
         f(i0 + 128 * k, v[k]);
+      after();
     }
   };
+  auto nothing = [] {};
 
   /* ---- the greatest logit */
   float mx = -INFINITY;
-  for_slice([&](unsigned, const float(&v)[4]) { mx = fmaxf(fmaxf(mx, fmaxf(v[0], v[1])), fmaxf(v[2], v[3])); }); // a NaN never wins
+  for_slice([&](unsigned, const float(&v)[4]) { mx = fmaxf(fmaxf(mx, fmaxf(v[0], v[1])), fmaxf(v[2], v[3])); }, nothing); // a NaN never wins
 #pragma unroll
   for (int o = 16; o; o >>= 1)
     mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
@@ -431,13 +441,13 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
   if (weight.fp32)
     weight.exact_from = fmaxf(weight.exact_from, head);
 
-  /* Logits from `from` up to `below` into the list of the first CTA; the others, four at a time, to f(logits, for each whether it is in
+  /* Logits that are `wanted` into the list of the first CTA; all, four at a time, to f(logits, for each whether it is in
    * the list); what f adds up in each slice goes to sh.sub of the first CTA. Returns how many are listed, ~0 if they are too many. Each CTA
    * has its own part of the list. */
   unsigned long long slice_sum = 0;
   unsigned n_above = 0;
   const unsigned room = SP_LIST / parts;
-  auto gather = [&](float from, float below, auto f) {
+  auto gather = [&](auto wanted, auto f, auto after) {
     if (tid == 0)
       sh.count = sh.n_above = 0;
     slice_sum = 0;
@@ -450,7 +460,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
       bool in[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        in[k] = v[k] >= from && v[k] < below;
+        in[k] = wanted(v[k]);
       f(v, in);
       if (in[0] || in[1] || in[2] || in[3])
 #pragma unroll
@@ -462,7 +472,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
               asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to_i + 4 * at), "r"(i + k) : "memory");
             }
           }
-    });
+    }, after);
     slice_sum = warp_sum(slice_sum);
     n_above = __reduce_add_sync(FULL, n_above);
     if (lane == 0 && n_above)
@@ -526,15 +536,22 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
 
   /* ---- the greatest logits listed, the others summed */
   const bool need_rest = whole || (has_p && !has_k);
-  unsigned listed = gather(head, INFINITY, [&](const float(&v)[4], const bool(&in)[4]) {
+  uint32_t sum_hi = 0, sum_lo = 0;
+  auto add_rest = [&](const float(&v)[4], const bool(&in)[4]) { // what is not listed is below exact_from
     if (!need_rest)
       return;
-    unsigned long long w[4]; // what is not listed is below exact_from
-    weight.in_fp32(v[0], v[1], &w[0], &w[1]);
-    weight.in_fp32(v[2], v[3], &w[2], &w[3]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      slice_sum += in[k] ? 0 : w[k];
+    for (int k = 0; k < 4; k += 2) {
+      uint32_t hi[2], lo[2];
+      weight.in_fp32(in[k] ? -INFINITY : v[k], in[k + 1] ? -INFINITY : v[k + 1], hi, lo);
+      sum_hi += hi[0] + hi[1];
+      sum_lo += lo[0] + lo[1];
+    }
+  };
+  unsigned listed = gather([&](float v) { return v >= head; }, add_rest, [&] {
+    if (need_rest)
+      slice_sum += Weigher::sum_of(sum_hi, sum_lo, 4 * AT);
+    sum_hi = sum_lo = 0;
   });
   const bool fits = listed != ~0u && weight.fp32; // else: by digits
   const bool all_listed = head == -3.402823466e38f;
@@ -901,14 +918,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
     /* ---- one more pass: the logits around the cut listed, those above summed */
     __syncthreads();
     const float from = sh.from, below = sh.upto;
-    listed = gather(from, below, [&](const float(&v)[4], const bool(&)[4]) {
+    listed = gather([&](float v) { return v >= from && v < below; }, [&](const float(&v)[4], const bool(&)[4]) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (v[k] >= below) {
           slice_sum += weight(v[k]);
           ++n_above;
         }
-    });
+    }, nothing);
     word = listed == ~0u || min_x >= below ? 2 : 0;
     if (word == 0) {
       if (part == 0) {
@@ -954,7 +971,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
           w4[k] = order_of(v[k]) ? w(v[k]) : 0;
         }
         f(k4, w4);
-      });
+      }, nothing);
     };
   };
   auto by_value = [](unsigned, float v) { return order_of(v); };
@@ -965,7 +982,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
       for (int k = 0; k < 4; ++k)
         if (which(i + k, v[k]))
           sum += weight(v[k]);
-    });
+    }, nothing);
     sum = warp_sum(sum);
     if (parts > 1) { // in every CTA
       if (lane < parts)

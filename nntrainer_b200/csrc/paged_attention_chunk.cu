@@ -349,7 +349,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PC_REGS_ROWS));
     /* ------------------------------ two threads per row ------------------------------ */
     const int t = warp / PC_ROW_WARPS, half = warp / 4 & 1, wrow = (warp & 3) * 32, row = wrow + lane, own = t * PC_ROWS + row;
-    const bool there = own < rows, busy = t * PC_ROWS + wrow < rows; // busy: a row of the warp is
+    const bool there = own < rows;
     const int p = there ? work[3] + token_of(own) : -1;
     constexpr int CH = HD / 8; // 16-byte pieces of a row
     uint4 w[CH / 2]; // 16 rows of the tile, all on their way together
@@ -392,7 +392,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       fence_after();
       const int j0 = sight.block(b_lo + j) * PC_KEYS;
       const bool all = j0 + PC_KEYS - 1 <= sight.lo && (j0 > sight.hi - sight.window || j0 + PC_KEYS <= a.first);
-      if (!all && busy) { // masked where they are: what follows need not know
+      if (!all) { // masked where they are: what follows need not know
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           const int k0 = j0 + 64 * half + 32 * c; // bit i: the row sees cache row k0 + i
@@ -415,7 +415,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         if (afresh) {
           float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-          for (int c = 0; c < (busy ? 2 : 0); ++c) {
+          for (int c = 0; c < 2; ++c) {
             uint32_t sr[32];
             tmem_ld32(s_at + 32 * c, sr);
             tmem_wait_ld();
@@ -449,14 +449,13 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         }
         const float base = m == -INFINITY ? 0.f : m - PAGED_LIFT;
         sum = 0.f;
-        if (busy)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t sr[32];
-            tmem_ld32(s_at + 32 * c, sr);
-            tmem_wait_ld();
-            sum += weights32<T>(sr, a.scale_log2, base, pr + 16 * c);
-          }
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sr[32];
+          tmem_ld32(s_at + 32 * c, sr);
+          tmem_wait_ld();
+          sum += weights32<T>(sr, a.scale_log2, base, pr + 16 * c);
+        }
         if (!rows_any(t, !came || (!afresh && sum > PC_MOST<T>)))
           break;
         if (rows_any(t, !came)) {
@@ -466,11 +465,9 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       }
       if (!ok)
         break;
-      if (busy) { // else: nobody asks for what comes of those rows
-        tmem_st32(s_at, pr);
-        l += sum;
-        tmem_wait_st();
-      }
+      tmem_st32(s_at, pr);
+      l += sum;
+      tmem_wait_st();
       fence_before();
       __syncwarp();
       if (lane == 0)

@@ -232,6 +232,40 @@ def test_counts_beyond_32_bits(be, new):
     assert torch.equal(c.attend(be, window=5, first_tokens=2 ** 32 + 5), want)
 
 
+@pytest.mark.parametrize("heads", [(192, 1, 64), (300, 2, 40), (260, 2, 128)])
+@pytest.mark.parametrize("new,ctx", [([1, 1], [100, 3]), ([3, 1, 5], [400, 1, 5])])
+def test_groups_wider_than_a_tile(be, heads, new, ctx):
+    c = Case(new, ctx, heads, F16, 16, seed=32)
+    c.check(c.attend(be))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [60, 2, 9]])
+@pytest.mark.parametrize("max_rows", [0, 1, 100, 1 << 29, (1 << 32) - 1])
+def test_any_expected_length_is_right(be, new, max_rows):
+    c = Case(new, [700, 90, 1100], (8, 2, 128), BF16, 32, seed=33)
+    c.check(c.attend(be, max_rows=max_rows))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_rows_in_front_of_the_first_sequence(be, new):
+    c = Case([new, new], [200, 90], (8, 2, 128), F16, 16, seed=34)
+    q = torch.cat([c.q.new_full((6, 8, 128), math.nan), c.q])
+    start = c.row_start + 6
+    out = torch.full_like(q, 5.0)
+    be.paged_attention(q, c.k, c.v, c.table, start, c.context, new, 200, out=out)
+    assert bool((out[:6] == 5).all())
+    c.check(out[6:])
+    cos, sin = tables(be, 200, 128)
+    x = torch.randn(q.shape[0], 12 * 128, device="cuda")
+    k, v = c.k.clone(), c.v.clone()
+    got = be.paged_append(x[:, :1024], x[:, 1024:1280], x[:, 1280:], k, v, c.table, start, c.context, new, cos, sin, q_out=torch.full_like(q, 5.0))
+    k2, v2 = c.k.clone(), c.v.clone()
+    want = be.paged_append(x[6:, :1024], x[6:, 1024:1280], x[6:, 1280:], k2, v2, c.table, c.row_start, c.context, new, cos, sin)
+    assert bool((got[:6] == 5).all()) and torch.equal(got[6:], want)
+    assert torch.equal(torch.nan_to_num(k), torch.nan_to_num(k2)) and torch.equal(torch.nan_to_num(v), torch.nan_to_num(v2))
+    be.device_status()
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_captured_and_replayed_with_other_contents(be, new):
     c = Case([new, new], [300, 200], (8, 2, 128), F16, 16, seed=8)

@@ -690,8 +690,7 @@ def paged_attention(q, kcache, vcache, page_table, row_start, context, max_new: 
     if window is not None and window < 0 or first_tokens < 0:
         raise ValueError("window and first_tokens are counts")
     if out is None:
-        out = q.new_empty((tokens, hq, hd))
-        ld_out = hq * hd
+        out, ld_out = torch.empty_like(q, memory_format=torch.contiguous_format), hq * hd
     else:
         ld_out, one, two = out.stride()
         if out.shape != q.shape or two != 1 or one != hd or out.dtype not in (t, torch.float32):
@@ -743,16 +742,17 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     rows = logits.numel() // n if n else 0
     if u.dtype is not f32 or u.numel() != rows or not u.is_contiguous():
         raise ValueError(f"u: need a contiguous fp32 tensor of {rows} elements")
+    flat = u if u.dim() == 1 else u.view(-1)
     if idx is None:
-        idx = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        idx = torch.empty_like(flat, dtype=torch.int32)
     else:
         _typed(idx, "out", torch.int32, rows)
     if idx_f is None:
-        idx_f = torch.empty_like(idx, dtype=f32)
+        idx_f = torch.empty_like(flat)
     else:
         _typed(idx_f, "out", f32, rows)
     if prob is None:
-        prob = torch.empty_like(idx_f)
+        prob = torch.empty_like(flat)
     else:
         _typed(prob, "out", f32, rows)
     rc = lib().nntr_cuda_sample_dev(

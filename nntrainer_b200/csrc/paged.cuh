@@ -37,13 +37,14 @@ struct PagedGeom {
 };
 
 /** A sequence's query rows [first, first + n) and the position of the first one; bad: the arrays contradict themselves or the
- *  bounds that came with them. Then no row outside q is in it, and no more than max_new. A negative position sees nothing. */
+ *  bounds that came with them. Then no row outside q is in it, and no more than max_new. A negative position sees nothing. Whatever the
+ *  arrays hold, -tokens <= pos and pos + n <= table_rows: a row up to a query's position that is not negative has an entry in the page table. */
 struct SeqRows {
   int first, n, pos;
   bool bad;
 };
 __device__ __forceinline__ SeqRows seq_rows(const PagedBatch &s, int lo, int hi, int given) { // row_start of it and of the next one, context
-  const int ctx = min(given, s.table_rows);
+  const int ctx = max(0, min(given, s.table_rows)); // from both sides: the difference below stays in 32 bits
   SeqRows r;
   r.first = min(max(lo, 0), s.tokens);
   const int end = min(max(hi, r.first), s.tokens);

@@ -140,31 +140,61 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-/* 32 scores of a row to probabilities 2^x, x = s * scale - base below 16, packed, and their sum. Some of the pairs are computed on the FMA pipes beside the special function unit, which alone would take as many clocks as a step's products: x = n + f
- * with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f by the polynomial of the least greatest relative error with value 1
- * at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent. There what is masked gets 2^-126 and not zero: of no
- * account beside a row's greatest probability, 2^6 or more. (A row that sees nothing has none: it is zero in the end.) */
+/* What a row's probabilities may be. The greatest is 2^LIFT when the maximum is taken that they refer to; other steps go by that maximum while
+ * no half of a row's step sums to more than MOST, so that each probability fits its type, and beyond it the step begins again. fp16: small
+ * ones of a long context stay out of the subnormal numbers. bf16 has the exponents of fp32: probabilities of at most 1 leave fp32 to the
+ * values, whose sums do not overflow unless rows * |value| does. FROM .. UPTO: exponents x of 2^x that are told apart; what is
+ * further down is as nothing beside 2^LIFT, what is further up, and a NaN, counts as UPTO, which is above MOST. */
+template <typename T> struct Weights;
+template <> struct Weights<__half> {
+  static constexpr float LIFT = 6.f, MOST = 32768.f, FROM = -48.f, UPTO = 16.f; // 2^-48: zero in fp16
+};
+template <> struct Weights<__nv_bfloat16> {
+  static constexpr float LIFT = -9.f, MOST = 1.f, FROM = -127.f, UPTO = 1.f;
+};
+
+__device__ __forceinline__ float fma_sat(float a, float b, float c) { // a b + c cut to 0 .. 1; NaN: 0
+  float d;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+/* 32 scores of a row to probabilities 2^x, x = s * scale - base, packed, and their sum. Some of the pairs are computed on the FMA pipes
+ * beside the special function unit, which alone would take as many clocks as a step's products: (UPTO - x) / (UPTO - FROM) cut to 0 .. 1
+ * (a power of two: nothing is rounded on the way back), x = n + f with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f by the
+ * polynomial of the least greatest relative error with value 1 at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent.
+ * The cut is what keeps n inside it: in a step that goes by an older maximum x may be anything. It costs nothing where clamping x from below and
+ * above took 2.4 % of the long chunks' time and a vote on the greatest x 5 %. What is masked is -inf: zero at FROM, also in bf16 (2^-127
+ * has the exponent 0 and no mantissa). */
 constexpr int PC_GROUP = 8, PC_BY_FMA = 3; // pairs that go step by step together, so many of them on the FMA pipes
 template <typename T>
 __device__ __forceinline__ float weights32(const uint32_t *s, float scale, float base, uint32_t *p) {
-  constexpr float MAGIC = 12582912.f;
   constexpr bool FOUR = MmaType<T>::bits == 0;
   constexpr int N = PC_BY_FMA;
+  constexpr float WIDE = Weights<T>::UPTO - Weights<T>::FROM, MAGIC = 12582912.f + Weights<T>::UPTO;
+  static_assert(WIDE == 64.f || WIDE == 128.f, "a power of two");
+  const float per = scale * (-1.f / WIDE), off = (base + Weights<T>::UPTO) * (1.f / WIDE);
   float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
   for (int g = 0; g < 16; g += PC_GROUP) {
     float2 x[PC_GROUP], t[PC_GROUP], f[PC_GROUP], q[PC_GROUP];
 #pragma unroll
     for (int i = 0; i < PC_GROUP; ++i) {
-      x[i] = make_float2(-base, -base);
-      fma2(x[i].x, x[i].y, __uint_as_float(s[2 * (g + i)]), __uint_as_float(s[2 * (g + i) + 1]), scale, scale);
+      const float s0 = __uint_as_float(s[2 * (g + i)]), s1 = __uint_as_float(s[2 * (g + i) + 1]);
+      if (i < N) {
+        x[i] = make_float2(fma_sat(s0, per, off), fma_sat(s1, per, off));
+      } else {
+        x[i] = make_float2(-base, -base);
+        fma2(x[i].x, x[i].y, s0, s1, scale, scale);
+      }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      x[i] = make_float2(fmaxf(x[i].x, -126.f), fmaxf(x[i].y, -126.f));
-      t[i] = add2(x[i].x, x[i].y, MAGIC, MAGIC);
-      f[i] = add2(t[i].x, t[i].y, -MAGIC, -MAGIC);
-      f[i] = add2(x[i].x, x[i].y, -f[i].x, -f[i].y);
+      t[i] = make_float2(MAGIC, MAGIC);
+      fma2(t[i].x, t[i].y, x[i].x, x[i].y, -WIDE, -WIDE);
+      const float2 n = add2(t[i].x, t[i].y, -MAGIC, -MAGIC); // less UPTO
+      f[i] = make_float2(-n.x, -n.y);
+      fma2(f[i].x, f[i].y, x[i].x, x[i].y, -WIDE, -WIDE);
       if constexpr (FOUR) {
         q[i] = make_float2(5.590642467794357e-2f, 5.590642467794357e-2f);
         fma2(q[i].x, q[i].y, f[i].x, f[i].y, 9.582853038422538e-3f, 9.582853038422538e-3f);
@@ -211,9 +241,6 @@ __device__ __forceinline__ bool rows_any(int t, bool v) {
                : "memory");
   return r != 0;
 }
-
-/* sum of a row thread's probabilities of a step up to which each fits its 16-bit type, and m may stay */
-template <typename T> constexpr float PC_MOST = MmaType<T>::bits == 0 ? 32768.f : 1e30f;
 
 /* Pair of tiles number `work` of the batch: its sequence and its place in it, by all lanes of a warp. False: there are fewer. What takes
  * longest comes first, so that it does not begin when the rest is done: in a sequence the last queries, which see most, and among up to
@@ -447,7 +474,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
           }
           unset = rows_any(t, there && m == -INFINITY);
         }
-        const float base = m == -INFINITY ? 0.f : m - PAGED_LIFT;
+        const float base = m == -INFINITY ? 0.f : m - Weights<T>::LIFT;
         sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -456,7 +483,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
           tmem_wait_ld();
           sum += weights32<T>(sr, a.scale_log2, base, pr + 16 * c);
         }
-        if (!rows_any(t, !came || (!afresh && sum > PC_MOST<T>)))
+        if (!rows_any(t, !came || !(afresh || sum <= Weights<T>::MOST)))
           break;
         if (rows_any(t, !came)) {
           ok = false;
@@ -491,7 +518,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
       if (parts == 1) {
         float total = l;
         if (a.sink && there)
-          total += ex2(a.sink[head_of(own, token_of(own))] * LOG2E - (m - PAGED_LIFT));
+          total += ex2(a.sink[head_of(own, token_of(own))] * LOG2E - (m - Weights<T>::LIFT));
         inv = m == -INFINITY || total == 0.f ? 0.f : 1.f / total;
       }
       // Rows by threads would be stored as 16 bytes of 32 rows at a time: they go through shared memory, where the tile's queries were, 16-byte
@@ -675,7 +702,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
             f = make_float4(f.x + w * v[k].x, f.y + w * v[k].y, f.z + w * v[k].z, f.w + w * v[k].w);
           }
         if (a.sink && big > -INFINITY)
-          total += ex2(a.sink[head] * LOG2E - (big - PAGED_LIFT));
+          total += ex2(a.sink[head] * LOG2E - (big - Weights<T>::LIFT));
         const float inv = total == 0.f ? 0.f : 1.f / total;
         const long long e = q_row(tok) * a.ld_out + (long long)head * g.hd + col;
         if (col < g.hd) {

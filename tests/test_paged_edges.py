@@ -47,3 +47,46 @@ def test_negative_contexts_see_nothing_and_are_told(be, new, context):
     assert bool((q[:new] == 0).all())
     own = c.table[0, :-(-100 // 16)].long()
     assert torch.equal(k[own], c.k[own]) and torch.equal(v[own], c.v[own])  # nothing of the first sequence is stored
+
+
+def late_peak(height, heads, dtype, new, batch=16, late=128):
+    """Flat scores but for one query row of each sequence, which has one key `height` (natural units) above all others: row `late` + b of
+    sequence b."""
+    c = Case([new] * batch, [400 + new] * batch, heads, dtype, 64, seed=80)
+    c.q[:] = 0
+    along = math.sqrt(height * math.sqrt(c.hd))
+    for b in range(batch):
+        c.K[b][:, :, 0] = 0
+        for r in range(0, c.ctx[b], c.page):
+            rows = c.K[b][r:r + c.page]
+            c.k[int(c.table[b, r // c.page]), :rows.shape[0]] = rows
+        key = c.K[b][late + b].clone()
+        key[:, 0] = along
+        put(c, b, late + b, k=key)
+        c.q[c.starts[b] + 5 * b % new, b % c.hq, 0] = along
+    return c
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads", [(2, 1, 64), (4, 2, 128), (2, 1, 96)])
+@pytest.mark.parametrize("new", [1, 64, 128])
+@pytest.mark.parametrize("height", [20, 60, 80, 84, 85, 86, 90, 95, 100, 130, 177, 200, 260, 300, 420, 600])
+def test_one_score_that_rises_late_and_alone(be, height, new, heads, dtype):
+    """At every place modulo 16 of a step whose rows all see everything, far above what the row's maximum was taken from."""
+    c = late_peak(height, heads, dtype, new)
+    c.check(c.attend(be))
+    c.check(c.attend(be, max_rows=64))  # not cut into parts
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads", [(2, 1, 64), (4, 1, 128)])
+@pytest.mark.parametrize("new", [2, 9, 40, 128])
+def test_values_out_of_sight_have_no_effect_whatever_their_size(be, new, heads, dtype):
+    """The last row is seen by the last query alone, row 100 by the first one alone (the window's begin): the others' results keep their bits."""
+    c = Case([new], [300], heads, dtype, 32, seed=81)
+    window = 300 - new + 1 - 100
+    want = c.attend(be, window=window)
+    for sign in (1, -1):
+        for row in (299, 100):
+            put(c, 0, row, v=sign * torch.finfo(dtype).max)
+        assert torch.equal(c.attend(be, window=window)[1:-1], want[1:-1])

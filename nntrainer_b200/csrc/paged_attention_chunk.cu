@@ -134,9 +134,9 @@ template <> struct MmaType<__nv_bfloat16> {
   static constexpr uint32_t bits = 1u << 7 | 1u << 10;
 };
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) { // NaN if one of them is
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -450,9 +450,13 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
             for (int i = 0; i < 32; i += 2)
               mx[i >> 1 & 1] = max3(mx[i >> 1 & 1], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
           }
-          *pair_own = fmaxf(mx[0], mx[1]) * a.scale_log2;
+          *pair_own = max3(mx[0], mx[1], mx[1]) * a.scale_log2;
           rows_sync(t);
-          const float big = fmaxf(*pair_own, *pair_other);
+          float big = max3(*pair_own, *pair_other, *pair_other);
+          if (!(big < INFINITY)) { // a score that is no number or infinite: the row's result is NaN, whichever pairs compute its weight
+            big = INFINITY;
+            l = NAN;
+          }
           const bool grown = big > m;
           if (__any_sync(FULL, grown)) {
             const float keep = grown ? ex2(m - big) : 1.f;

@@ -90,3 +90,23 @@ def test_values_out_of_sight_have_no_effect_whatever_their_size(be, new, heads, 
         for row in (299, 100):
             put(c, 0, row, v=sign * torch.finfo(dtype).max)
         assert torch.equal(c.attend(be, window=window)[1:-1], want[1:-1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads", [(2, 1, 64), (4, 1, 128)])
+@pytest.mark.parametrize("new", [1, 64, 128])
+@pytest.mark.parametrize("at", [0, 130, 270])
+def test_a_key_that_is_no_number_shows(be, at, new, heads, dtype):
+    """Wherever it lies in a step: the results of the queries that see it are not finite (those of 128 new tokens in front of it do not)."""
+    c = Case([new] * 16, [400] * 16, heads, dtype, 16, seed=82)
+    for b in range(16):
+        put(c, b, at + b, k=math.nan)
+    sees = torch.arange(400 - new, 400, device="cuda") >= at + torch.arange(16, device="cuda")[:, None]
+    for out in (c.attend(be), c.attend(be, max_rows=64)):
+        assert torch.equal(torch.isfinite(out).view(16, new, -1), ~sees[..., None].expand(16, new, c.hq * c.hd))
+    c = Case([new] * 16, [400] * 16, heads, dtype, 16, seed=82)
+    want = c.attend(be)
+    for b in range(16):
+        put(c, b, 399, k=math.nan)  # the last query's own row
+    got = c.attend(be).view(16, new, -1)
+    assert torch.equal(got[:, :-1], want.view(16, new, -1)[:, :-1]) and not bool(torch.isfinite(got[:, -1]).any())

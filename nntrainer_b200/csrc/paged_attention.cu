@@ -8,8 +8,7 @@
  *   out = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m)), m = max_j s_j; zeros where nothing is seen
  *
  * Scores, maxima, sums and results are fp32. The probabilities are rounded to the cache's 16-bit type, the operand type of the
- * tensor cores (2^-11 or 2^-8 of each, which the sum over the rows averages out); the greatest is kept near 2^6, so
- * that the small ones of a long context stay out of the subnormal numbers of fp16.
+ * tensor cores (2^-11 or 2^-8 of each, which the sum over the rows averages out); what they may be: Weights in paged_attention.cuh.
  */
 #include "cluster.cuh"
 #include "paged_attention.cuh"
@@ -18,7 +17,6 @@
 
 #include <algorithm>
 #include <climits>
-#include <type_traits>
 
 namespace nntr {
 
@@ -232,7 +230,6 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
 #pragma unroll
   for (int c = 0; c < HD / 8; ++c)
     o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-  constexpr float MOST = std::is_same<T, __half>::value ? 32768.f : 1e30f; // sum of a lane's probabilities up to which each fits its type
   for (int i = 0; i < n_mine; ++i) {
     fetch(i + Cfg::STAGES - 1);
     if (!mbar_wait_warp(bars + 8 * (i % Cfg::STAGES), i / Cfg::STAGES & 1, abort_flag, &g_paged_attn_status, PD_POLLS, 2048))
@@ -304,14 +301,14 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) { // the lane's two rows
-        const float base = m[k] == -INFINITY ? 0.f : m[k] - PAGED_LIFT; // nothing seen yet: all weights are 2^(-inf)
+        const float base = m[k] == -INFINITY ? 0.f : m[k] - Weights<T>::LIFT; // nothing seen yet: all weights are 2^(-inf)
         const float p0 = ex2(fmaf(sc[0][2 * k], a.scale_log2, -base)), p1 = ex2(fmaf(sc[0][2 * k + 1], a.scale_log2, -base)),
                     p2 = ex2(fmaf(sc[1][2 * k], a.scale_log2, -base)), p3 = ex2(fmaf(sc[1][2 * k + 1], a.scale_log2, -base));
         sum[k] = (p0 + p1) + (p2 + p3);
         pf[k] = pack2<T>(p0, p1);
         pf[k + 2] = pack2<T>(p2, p3);
       }
-      if (afresh || !__any_sync(FULL, sum[0] > MOST || sum[1] > MOST))
+      if (afresh || !__any_sync(FULL, sum[0] > Weights<T>::MOST || sum[1] > Weights<T>::MOST))
         break;
     }
     l[0] += sum[0];
@@ -357,7 +354,7 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
     const int flat = tile * 16 + row, head = h * G + flat % G;
     float total = j.l;
     if (a.sink && j.m > -INFINITY)
-      total += ex2(a.sink[head] * LOG2E - (j.m - PAGED_LIFT));
+      total += ex2(a.sink[head] * LOG2E - (j.m - Weights<T>::LIFT));
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const float4 f = make_float4(j.sum.x * inv, j.sum.y * inv, j.sum.z * inv, j.sum.w * inv);
     const long long e = (r.first + flat / G) * a.ld_out + (long long)head * g.hd + col;

@@ -29,8 +29,20 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-/** log2 of what a row's greatest probability is when its maximum is taken */
-constexpr float PAGED_LIFT = 6.f;
+/* What a row's probabilities may be. The greatest is 2^LIFT when the maximum is taken that they refer to; the rows behind go by that maximum
+ * while no thread's sum of a step (a lane's four, or half a row of a step) is above MOST, so that each probability fits its type, and beyond it
+ * the step begins again. So a row's greatest probability lies between 2^LIFT and MOST, and so does the exponent that a sink meets. fp16: the small
+ * ones of a long context stay out of the subnormal numbers. bf16 has the exponents of fp32: probabilities of at most 1 leave those to the
+ * values, whose sums overflow only where rows * |value| does. FROM .. UPTO: exponents x of 2^x that the polynomial of
+ * paged_attention_chunk.cu tells apart; what is further down is as nothing beside 2^LIFT, what is further up, and a NaN, counts as UPTO, which is
+ * above MOST. */
+template <typename T> struct Weights;
+template <> struct Weights<__half> {
+  static constexpr float LIFT = 6.f, MOST = 32768.f, FROM = -48.f, UPTO = 16.f; // 2^-48: zero in fp16
+};
+template <> struct Weights<__nv_bfloat16> {
+  static constexpr float LIFT = -9.f, MOST = 1.f, FROM = -127.f, UPTO = 1.f;
+};
 
 /* Blocks of KEYS cache rows that hold what a tile of queries at positions lo .. hi sees: those of the first tokens, then the window's.
  * A row in none of the queries' sight counts as not there: it may hold anything. */

@@ -140,19 +140,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) { // NaN if one
   return d;
 }
 
-/* What a row's probabilities may be. The greatest is 2^LIFT when the maximum is taken that they refer to; other steps go by that maximum while
- * no half of a row's step sums to more than MOST, so that each probability fits its type, and beyond it the step begins again. fp16: small
- * ones of a long context stay out of the subnormal numbers. bf16 has the exponents of fp32: probabilities of at most 1 leave fp32 to the
- * values, whose sums do not overflow unless rows * |value| does. FROM .. UPTO: exponents x of 2^x that are told apart; what is
- * further down is as nothing beside 2^LIFT, what is further up, and a NaN, counts as UPTO, which is above MOST. */
-template <typename T> struct Weights;
-template <> struct Weights<__half> {
-  static constexpr float LIFT = 6.f, MOST = 32768.f, FROM = -48.f, UPTO = 16.f; // 2^-48: zero in fp16
-};
-template <> struct Weights<__nv_bfloat16> {
-  static constexpr float LIFT = -9.f, MOST = 1.f, FROM = -127.f, UPTO = 1.f;
-};
-
 __device__ __forceinline__ float fma_sat(float a, float b, float c) { // a b + c cut to 0 .. 1; NaN: 0
   float d;
   asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

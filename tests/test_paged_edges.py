@@ -110,3 +110,16 @@ def test_a_key_that_is_no_number_shows(be, at, new, heads, dtype):
         put(c, b, 399, k=math.nan)  # the last query's own row
     got = c.attend(be).view(16, new, -1)
     assert torch.equal(got[:, :-1], want.view(16, new, -1)[:, :-1]) and not bool(torch.isfinite(got[:, -1]).any())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads", [(2, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("new", [1, 64])
+@pytest.mark.parametrize("height", [5, 30, 60, 66])
+def test_large_values_behind_a_score_that_rises_late(be, height, new, heads, dtype):
+    """Weights refer to a maximum that was taken before the score rose: their products with the values stay inside fp32."""
+    c = late_peak(height, heads, dtype, new)
+    for b in range(16):
+        put(c, b, 128 + b, v=1e12 if dtype == BF16 else 6e4)
+    c.check(c.attend(be))
+    c.check(c.attend(be, max_rows=64))

@@ -78,6 +78,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) { // NaN if one of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 /* Parts of a row's result, four of O's columns, joined one after the other, up to four on their way at a time: load(i, &v, &ml). */
 struct Joined {
   float4 sum;
@@ -277,15 +283,19 @@ paged_attention_few_kernel(const __grid_constant__ CUtensorMap kmap, const __gri
         float mx[2], keep[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-          mx[k] = fmaxf(fmaxf(sc[0][2 * k], sc[0][2 * k + 1]), fmaxf(sc[1][2 * k], sc[1][2 * k + 1]));
+          mx[k] = max_nan(max_nan(sc[0][2 * k], sc[0][2 * k + 1]), max_nan(sc[1][2 * k], sc[1][2 * k + 1]));
 #pragma unroll
         for (int d = 1; d < 4; d *= 2)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            mx[k] = fmaxf(mx[k], __shfl_xor_sync(FULL, mx[k], d));
+            mx[k] = max_nan(mx[k], __shfl_xor_sync(FULL, mx[k], d));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float big = fmaxf(m[k], mx[k] * a.scale_log2);
+          float big = max_nan(m[k], mx[k] * a.scale_log2);
+          if (!(big < INFINITY)) { // a score that is no number or infinite, maybe the only one: the row's result is NaN
+            big = INFINITY;
+            l[k] = NAN;
+          }
           keep[k] = big > m[k] ? ex2(m[k] - big) : 1.f;
           m[k] = big;
           l[k] *= keep[k];

@@ -123,3 +123,21 @@ def test_large_values_behind_a_score_that_rises_late(be, height, new, heads, dty
         put(c, b, 128 + b, v=1e12 if dtype == BF16 else 6e4)
     c.check(c.attend(be))
     c.check(c.attend(be, max_rows=64))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads", [(2, 1, 64), (8, 1, 128)])
+@pytest.mark.parametrize("ctx", [1, 2, 17, 40])
+@pytest.mark.parametrize("kind", ["nan", "inf"])
+def test_nothing_but_keys_that_are_no_numbers_shows(be, kind, ctx, heads, dtype):
+    """A row that has no finite score at all, or whose score is +inf; the sequence beside it is not affected."""
+    c = Case([1, 1], [ctx, 60], heads, dtype, 16, seed=85)
+    c.q[:, :, 0] = 1
+    want = c.attend(be)[1]
+    for r in range(ctx):
+        k = c.K[0][r].clone()
+        k[:, 0] = math.nan if kind == "nan" else math.inf
+        put(c, 0, r, k=k)
+    for kw in (dict(), dict(sink=c.sinks), dict(max_rows=1)):
+        out = c.attend(be, **kw)
+        assert bool(torch.isnan(out[0]).all()) and (kw.get("sink") is not None or torch.equal(out[1], want))

@@ -59,6 +59,7 @@ struct Sight {
   }
   __device__ __forceinline__ int block(int i) const { return i < head_blocks ? i : i - head_blocks + first_block; }
   __device__ __forceinline__ bool row_read(int j) const { return j <= hi && (j >= from || j < first); } // by one query at least
+  __device__ __forceinline__ bool any_read(int j, int n) const { return j <= hi && (j + n > from || j < first); } // of the rows j .. j + n - 1
 };
 
 /* chunks of queries (paged_attention_chunk.cu) */

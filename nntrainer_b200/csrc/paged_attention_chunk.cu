@@ -11,6 +11,7 @@
  *   warps 16, 17    one for each tile; a thread issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as
  *                   it lies, dimensions contiguous). While one tile's probabilities are computed the other tile's products run.
  *   warp 18         TMA copies of K and V tiles through one ring of slots: a box per page (128 rows of it at most) and 64 dimensions.
+ *   warp 19         tells of pages and lengths that contradict the bounds.
  * Tensor memory: S (P) 128 columns a tile, O head_dim columns a tile.
  * Few tiles: the CTAs of a cluster share a pair of tiles along the cache rows and join through each other's shared memory.
  * Every wait is bounded (pipeline.cuh).
@@ -51,7 +52,7 @@ constexpr int PC_ROWS = 128; // of a tile: the MMA's M, lanes of tensor memory
 constexpr int PC_KEYS = 128; // cache rows of a step
 constexpr int PC_ROW_WARPS = 8; // of a tile: two threads per row, each with one half of a step's cache rows
 constexpr int PC_MMA_WARP = 2 * PC_ROW_WARPS, PC_COPY_WARP = PC_MMA_WARP + 2;
-constexpr int PC_THREADS = (PC_MMA_WARP + 4) * 32; // the last warp only makes the group of four whole
+constexpr int PC_THREADS = (PC_MMA_WARP + 4) * 32;
 /* Registers of a thread: 96 at launch (640 * 96 of the 65536); the last group gives some to the others: 4 * 104 + 64 = 5 * 96. */
 constexpr int PC_REGS_ROWS = 104, PC_REGS_REST = 64;
 constexpr uint32_t PC_POLLS = 1u << 22;
@@ -638,8 +639,6 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
           const int given = __ldg(s.table + (size_t)seq * s.ld_table + (at >> g.page_shift));
           if ((unsigned)given < (unsigned)g.n_pages)
             page = given;
-          else
-            atomicExch(&g_paged_chunk_status, NNTR_CUDA_ERR_INVALID);
         }
       }
       const int slot = i % Cfg::SLOTS, use = i / Cfg::SLOTS;
@@ -652,7 +651,18 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __g
         tma_box4(sbase + Cfg::OFF_RING + slot * Cfg::TILE + half * (PC_KEYS * 128) + at_row * 128, i & 1 ? &vmap : &kmap, half * 64, row, h, page,
                  FULL_BAR(slot));
     }
-    if (blockIdx.x == 0) // one that has no rows has no CTA either
+    __syncwarp();
+  } else {
+    /* ------------------------------ contradictions ------------------------------ */
+    // Pages outside the pool that a query sees a row of; others may have been given back. Apart from the copies, whose way to a page is short so.
+    const int box_shift = min(g.page_shift, 7), each = PC_KEYS >> box_shift;
+    for (int i = lane; i < steps * each; i += 32) {
+      const int at = sight.block(b_lo + i / each) * PC_KEYS + (i % each << box_shift);
+      if (sight.any_read(at, 1 << box_shift) &&
+          (unsigned)__ldg(s.table + (size_t)seq * s.ld_table + (at >> g.page_shift)) >= (unsigned)g.n_pages)
+        atomicExch(&g_paged_chunk_status, NNTR_CUDA_ERR_INVALID);
+    }
+    if (blockIdx.x == 0) // a sequence that has no rows has no CTA either
       for (int b = lane; b < s.batch; b += 32)
         if (seq_rows(s, b).bad)
           atomicExch(&g_paged_chunk_status, NNTR_CUDA_ERR_INVALID);

@@ -141,3 +141,23 @@ def test_nothing_but_keys_that_are_no_numbers_shows(be, kind, ctx, heads, dtype)
     for kw in (dict(), dict(sink=c.sinks), dict(max_rows=1)):
         out = c.attend(be, **kw)
         assert bool(torch.isnan(out[0]).all()) and (kw.get("sink") is not None or torch.equal(out[1], want))
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 256])
+@pytest.mark.parametrize("new", [1, 20, 65, 200])
+@pytest.mark.parametrize("window,first", [(100, 4), (100, 0), (33, 40), (300, 1)])
+def test_pages_that_nobody_sees_may_be_given_back(be, window, first, new, page):
+    """Page table entries of -1 between the first tokens and the window are no contradiction."""
+    be.check(be.lib().nntr_cuda_clear_device_status())
+    c = Case([new, new, 1], [1500, 1111, 900], (8, 2, 64), F16, page, seed=83)
+    kw = dict(window=window, first_tokens=first)
+    gone = 0
+    for b, (n, ctx) in enumerate(zip(c.new, c.ctx)):
+        oldest = max(0, ctx - n - window + 1)
+        for slot in range(-(-ctx // page)):
+            if (slot + 1) * page <= oldest and slot * page >= min(first, oldest):
+                c.table[b, slot] = -1
+                gone += 1
+    assert gone > 0
+    c.check(c.attend(be, **kw), **kw)
+    be.device_status()

@@ -89,7 +89,7 @@ struct Weigher {
     c_lo = (float)(c - (double)c_hi);
     m_hi = (float)(rint(m * 8.0) * 0.125); // plus a small whole number it is exact
     m_lo = (float)(m - (double)m_hi);
-    fp32 = fabs(m) < 1048576.0;
+    fp32 = fabs(m) < 1048576.0 && c <= 3.402823466e38; // with a greatest logit of 0 m says nothing about c
     least = (float)(top - 60.0 / c);
     if (!fp32) { // it is not: few logits are that large against the temperature
       c_hi = c_lo = m_lo = least = 0.f; // what is in no order weighs 2^-60

@@ -408,7 +408,7 @@ int nntr_cuda_copy_pages_dev(void *base, unsigned arrays, int64_t array_bytes, i
  *  temperature or top_p that is not above 0 means the greatest logit.
  *  idx_out (uint32) and / or idx_out_f (as a float) may be NULL; prob_out, or NULL: the token's weight over the kept ones' sum.
  *  temperature: at most 1e30. The greatest weights (from 2^-14 of the greatest one on, a few thousand of them) are double precision, the
- *  others fp32 to 2^-22; sums are exact in whole multiples of 2^-44 of the greatest weight: the token does not depend on how the work is
+ *  others fp32 to 2^-22; sums are exact in whole multiples of 2^-44 of the greatest weight (2^-43 where there are 2^20 logits): the token does not depend on how the work is
  *  split, and a draw is another than exact arithmetic's only where u or a threshold falls within about 2^-21 of a border. Up to 2^20
  *  logits, 65535 rows. */
 int nntr_cuda_sample_dev(const float *logits, int64_t rows, int64_t n, int64_t ld, const float *u, double temperature, unsigned top_k,

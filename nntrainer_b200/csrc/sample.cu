@@ -7,7 +7,7 @@
  * them are kept, of these the shortest prefix whose weights reach top_p times their sum, of these those with w_i >= min_p. The token is
  * the first kept one, in ascending order of the index, up to which the kept weights exceed u times their sum.
  *
- * A token is right or wrong, so the sums must not depend on their order: weights are whole multiples of 2^-44 in 64 bits. The ones that
+ * A token is right or wrong, so the sums must not depend on their order: weights are whole multiples of 2^-44 (2^20 logits: 2^-43) in 64 bits. The ones that
  * count most (a few thousand of the greatest logits, down to 2^-14 of the greatest weight) are computed in double precision, the rest
  * of the row in fp32 to 2^-22 of themselves.
  *
@@ -39,7 +39,7 @@ constexpr int SP_AROUND = 4400;            // ... and around a cut further down:
 constexpr int SP_FEW = 128;                // tokens that are compared each with each
 constexpr int SP_BINS = 512;               // of the estimate, over 46 powers of two of the weight
 constexpr int SP_EVERY = 8;                // every eighth block of 128 logits is in it
-constexpr double SP_ONE = 17592186044416.0; // 2^44: 2^20 logits of the greatest weight stay in 64 bits
+constexpr double SP_ONE = 17592186044416.0; // 2^44: fewer than 2^20 logits of the greatest weight stay in 64 bits
 constexpr float SP_HIGH = 6.f, SP_LOW = 1.5f / 2097152.f; // the last bit of the one plus a weight is 2^-21, of the other plus up to 2^-22 either way 2^-44
 constexpr double SP_EXACT_NATS = 9.7;      // (x - max) / T of the lightest token in double precision: 2^-14
 constexpr unsigned SP_MAX_N = 1u << 20;
@@ -80,15 +80,17 @@ struct Weigher {
   float mx, exact_from, least; // the greatest logit; from here up in double precision; logits further down weigh as little as this one, nothing
   bool fp32;            // others in fp32; else all in double precision
   double top, per_t;
+  unsigned n; // logits
   float c_hi, c_lo, m_hi, m_lo; // log2(e) / T, and times the greatest logit, each as a sum of two
 
-  __device__ __forceinline__ Weigher(float mx_, double t) : mx(mx_), top(mx_), per_t(1.0 / t) {
+  __device__ __forceinline__ Weigher(float mx_, double t, unsigned n_) : mx(mx_), top(mx_), per_t(1.0 / t), n(n_) {
     exact_from = fmaxf((float)(top - SP_EXACT_NATS * t), -3.402823466e38f);
     const double c = 1.4426950408889634 / t, m = c * top;
     c_hi = (float)c;
     c_lo = (float)(c - (double)c_hi);
     m_hi = (float)(rint(m * 8.0) * 0.125); // plus a small whole number it is exact
     m_lo = (float)(m - (double)m_hi);
+    m_hi += n == SP_MAX_N ? 1.f : 0.f;
     fp32 = fabs(m) < 1048576.0 && c <= 3.402823466e38; // with a greatest logit of 0 m says nothing about c
     least = (float)(top - 60.0 / c);
     if (!fp32) { // it is not: few logits are that large against the temperature
@@ -97,8 +99,10 @@ struct Weigher {
       exact_from = -3.402823466e38f;
     }
   }
+  /* the greatest weight: half of 2^44 where there are as many logits as can be, so that their sum is not 2^64 */
+  __device__ __forceinline__ double one() const { return n == SP_MAX_N ? SP_ONE / 2 : SP_ONE; }
   __device__ __forceinline__ double exactly(float x) const { return x == mx ? 1.0 : x > -INFINITY ? exp(((double)x - top) * per_t) : 0.0; }
-  __device__ __forceinline__ unsigned long long exact_one(float x) const { return __double2ull_rn(exactly(x) * SP_ONE); }
+  __device__ __forceinline__ unsigned long long exact_one(float x) const { return __double2ull_rn(exactly(x) * one()); }
   /* Two logits, their weights rounded to whole multiples of 2^-44: of 2^-21 in the low bits of w + 6, what is left of that, of 2^-44 in those
    * of the rest + 1.5 * 2^-21. So most of it is fp32, two operations in one instruction, and sums of weights are sums of words. (64-bit shifts,
    * comparisons and selections run at half the rate: with them the reading of 128 rows took 1.6 times as long.) */
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
   }
   if (!(top_p > 0.0))
     top_k = 1;
-  Weigher weight(mx, temperature);
+  Weigher weight(mx, temperature, a.n);
   const bool has_k = top_k > 0 && top_k < a.n, has_p = top_p > 0.0 && top_p < 1.0;
   const bool whole = !has_k && !has_p && !(min_p > 0.0); // every token is kept
   if (tid == SP_THREADS - 1)
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
         const unsigned m = __ballot_sync(FULL, w > 0 && upto >= goal);
         if (m) {
           if (lane == __ffs(m) - 1)
-            tell(i, weight.exactly(x[i]) * SP_ONE / (double)total);
+            tell(i, weight.exactly(x[i]) * weight.one() / (double)total);
           break;
         }
         run = __shfl_sync(FULL, upto, 31);
@@ -751,7 +755,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
       }
       const unsigned long long total = warp_sum(held), goal = goal_of(total);
       if (held && upto >= goal && upto - held < goal)
-        tell(id, weight.exactly(value_of(o)) * SP_ONE / (double)total);
+        tell(id, weight.exactly(value_of(o)) * weight.one() / (double)total);
       return true;
     }
     const bool there = tid < n;
@@ -788,7 +792,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
         upto += ij <= id ? wj : 0;
       }
       if (mine && w && upto >= goal && upto - w < goal)
-        tell(id, weight.exactly(value_of(o)) * SP_ONE / (double)total);
+        tell(id, weight.exactly(value_of(o)) * weight.one() / (double)total);
     }
     return true;
   };
@@ -905,7 +909,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a) {
         return kept(sh.i[i], sh.x[i]) ? sh.w[i] : 0;
       }), &before, &at);
       if (tid == 0)
-        tell(id, weight.exactly(x[id]) * SP_ONE / (double)total);
+        tell(id, weight.exactly(x[id]) * weight.one() / (double)total);
     }
   } else if (open) {
     cluster_sync();

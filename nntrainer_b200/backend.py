@@ -849,11 +849,19 @@ class PagedCache:
                     max_rows=max(self._seqs[s][0] for s in seqs))
 
     def fork(self, seq: int, n: int = 1) -> list:
-        """n new sequences with the rows of ``seq``."""
+        """n new sequences with the rows of ``seq``, which have to be in the cache by then: those that are only reserved are not copied.
+        MemoryError, or the error of a copy that is refused, with nothing changed."""
         rows, pages = self._seqs[seq]
         full = rows // self.page_size
         part = pages[full:]  # the page that the rows end in, if they end inside one
         fresh = self._take(n * len(part))
+        try:
+            self._copy(part * n, fresh)
+        except BaseException:  # refused (another device than the current one, a graph being captured): nothing has changed
+            for p in fresh:
+                self._refs[p] = 0
+            self._free += reversed(fresh)
+            raise
         out = []
         for i in range(n):
             s = self.new()
@@ -862,7 +870,6 @@ class PagedCache:
             for p in pages[:full]:
                 self._refs[p] += 1
             out.append(s)
-        self._copy(part * n, fresh)
         return out
 
     def free(self, seq: int) -> None:

@@ -41,3 +41,16 @@ def test_a_fork_on_a_cache_that_no_launch_can_reach_changes_nothing():
     with pytest.raises(ValueError):
         c.compact()
     assert c.pages(b) == pages and c._refs == refs and c.free_pages == 3
+
+
+def test_the_two_forms_of_the_structures_agree():
+    """The calls pack nntr_paged_cache and nntr_paged_batch in one go; capi declares their fields."""
+    c = be._PAGED_CACHE.pack(8, 2, 64, 30, 16, 1000, 1 << 40, 0x7f0011223344, 0x7f5566778899)
+    want = capi.PagedCache(8, 2, 64, 30, 16, 1000, 1 << 40, 0x7f0011223344, 0x7f5566778899)
+    assert len(c) == C.sizeof(capi.PagedCache) and c == bytes(want)
+    b = be._PAGED_BATCH.pack(3, 70, 60, 4000, 250, 0x7f0011223344, 0x7f5566778899, 0x7faabbccddee)
+    want = capi.PagedBatch(3, 70, 60, 4000, 250, 0x7f0011223344, 0x7f5566778899, 0x7faabbccddee)
+    assert len(b) == C.sizeof(capi.PagedBatch)
+    for name, kind in capi.PagedBatch._fields_:  # padding between them holds nothing
+        at = getattr(capi.PagedBatch, name)
+        assert b[at.offset:at.offset + at.size] == bytes(want)[at.offset:at.offset + at.size], name

@@ -74,7 +74,7 @@ struct AppendArgs {
   void *q_out, *kcache, *vcache;
   long long ld_q, ld_kv, ld_out;
   float eps;
-  int table_rows, chunks; // chunks: CTAs of a token
+  int table_rows, chunks, ctas; // chunks: CTAs of a token; ctas: ranges of tokens. One more CTA tells of sequences that contradict the bounds
 };
 
 __device__ __forceinline__ float4 load4(const float *p, bool vec) {
@@ -89,12 +89,13 @@ template <typename T> __device__ __forceinline__ void store4(T *p, const float4 
  * few instructions go into an element: what a head's lanes need to know of it is computed once, mean and root by a multiplication and the
  * approximate reciprocal root (2^-22). VEC: rows, gammas and tables are 16-byte aligned.
  * 3760 tokens of 32 + 2 x 8 heads of 128 (139 MB beside the tables): 31.5 us, 4.4 TB/s; one head a lane group, CTAs by heads and
- * divisions 36.2. 64 tokens: 3.3 us, the latency of a launch, of one head's loads and of its sum. */
+ * divisions 36.2. What is left is waiting: a lane group asks for a token's rows when it is through with the one in front (issue slots 63 %, HBM
+ * 44 %). 64 tokens: 3.3 us, the latency of a launch, of one head's loads and of its sum. */
 template <typename T, int U, bool VEC>
 __global__ void __launch_bounds__(PA_THREADS, U == 1 ? 5 : 4) paged_append_kernel(AppendArgs a, PagedGeom g, PagedBatch s) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, l = threadIdx.x % PA_LANES;
-  const int ctas = gridDim.x / a.chunks, cta = blockIdx.x / a.chunks, head0 = (blockIdx.x % a.chunks) * (PA_HEADS * U) + threadIdx.x / PA_LANES;
+  const int ctas = a.ctas, cta = blockIdx.x / a.chunks, head0 = (blockIdx.x % a.chunks) * (PA_HEADS * U) + threadIdx.x / PA_LANES;
   const int half = g.hd / 2, e = 4 * l;
   const float *src[U], *gamma[U];
   T *to[U]; // row 0 of the caches or of the result
@@ -114,6 +115,12 @@ __global__ void __launch_bounds__(PA_THREADS, U == 1 ? 5 : 4) paged_append_kerne
   }
   const float per_dim = 1.0f / (float)g.hd;
   pdl_wait();
+  if (cta >= ctas) { // those too that no token belongs to
+    for (int b = threadIdx.x; b < s.batch; b += PA_THREADS)
+      if (seq_rows(s, b).bad)
+        atomicExch(&g_paged_cache_status, NNTR_CUDA_ERR_INVALID);
+    return;
+  }
   int seq = 0;
   SeqRows r = {0, 0, 0, false};
   const int last = (int)((long long)s.tokens * (cta + 1) / ctas);
@@ -133,8 +140,6 @@ __global__ void __launch_bounds__(PA_THREADS, U == 1 ? 5 : 4) paged_append_kerne
       if (seq >= s.batch)
         return; // behind the last sequence: left as it is
       r = seq_rows(s, seq);
-      if (r.bad && threadIdx.x == 0)
-        atomicExch(&g_paged_cache_status, NNTR_CUDA_ERR_INVALID);
     }
     const int i = token - r.first, pos = r.pos + i;
     if (i < 0 || i >= r.n)
@@ -205,7 +210,7 @@ int launch_paged_append(const nntr_paged_cache *c, const nntr_paged_batch *b, co
                      (long long)ld_q, (long long)ld_kv, (long long)ld_out);
   if (table_rows > 0x7fffffffu)
     table_rows = 0x7fffffffu;
-  AppendArgs a = {q, k, v, q_gamma, k_gamma, cos_tab, sin_tab, q_out, c->kcache, c->vcache, ld_q, ld_kv, ld_out, eps, (int)table_rows, 0};
+  AppendArgs a = {q, k, v, q_gamma, k_gamma, cos_tab, sin_tab, q_out, c->kcache, c->vcache, ld_q, ld_kv, ld_out, eps, (int)table_rows, 0, 0};
   uintptr_t low = 0;
   for (const float *p : {q, k, v, q_gamma, k_gamma, cos_tab, sin_tab})
     low |= reinterpret_cast<uintptr_t>(p);
@@ -215,11 +220,12 @@ int launch_paged_append(const nntr_paged_cache *c, const nntr_paged_batch *b, co
   const int groups = (g.hq + 2 * g.hkv + PA_HEADS - 1) / PA_HEADS;
   const int each = (long long)s.tokens * groups < 16ll * sm_count() ? 1 : groups % 3 == 0 || groups > 4 ? 3 : groups % 2 == 0 ? 2 : groups;
   a.chunks = (groups + each - 1) / each;
-  const int at_once = (each == 1 ? 5 : 4) * sm_count(), ctas = std::min(s.tokens, std::max(1, at_once / a.chunks));
+  const int at_once = (each == 1 ? 5 : 4) * sm_count() - 1;
+  a.ctas = std::min(s.tokens, std::max(1, at_once / a.chunks));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   launch_cfg(cfg, attr, flags, st);
-  cfg.gridDim = dim3((unsigned)(ctas * a.chunks));
+  cfg.gridDim = dim3((unsigned)(a.ctas * a.chunks + 1));
   cfg.blockDim = dim3(PA_THREADS);
   auto launch = [&](auto value) {
     using T = decltype(value);

@@ -161,3 +161,41 @@ def test_pages_that_nobody_sees_may_be_given_back(be, window, first, new, page):
     assert gone > 0
     c.check(c.attend(be, **kw), **kw)
     be.device_status()
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("pad", [0, 40, 300])
+@pytest.mark.parametrize("what", ["backwards", "behind", "negative", "too many", "fewer rows", "no rows, negative", "none"])
+def test_append_tells_what_attention_tells(be, what, pad, new):
+    """Contradictions of sequences that no token belongs to, too, wherever they stand among sequences of padding."""
+    be.check(be.lib().nntr_cuda_clear_device_status())
+    c = Case([new, new], [100, 120], (8, 2, 64), F16, 16, seed=86, extra_rows=3, junk=0.0)
+    cos, sin = tables(be, 120, 64)
+    start, context = c.row_start.tolist() + [2 * new] * pad, [100, 120] + [0] * pad
+    table = torch.cat([c.table, torch.full((pad, c.table.shape[1]), -1, dtype=I32, device="cuda")])
+    if what == "backwards":
+        start[:3] = [new, 0, 2 * new]
+    elif what == "behind":
+        start[-1] = c.tokens + 1
+    elif what == "negative":
+        start[0] = -7
+    elif what == "too many":
+        start[1] += 1
+    elif what == "fewer rows":
+        context[0] = new - 1
+    elif what == "no rows, negative":
+        start, context, table = start + [start[-1]], context + [-1], torch.cat([table, table[:1]])
+    start, context = (torch.tensor(v, dtype=I32, device="cuda") for v in (start, context))
+    qkv = torch.randn(c.tokens, 12 * 64, device="cuda")
+
+    def told():
+        if what == "none":
+            return be.device_status()
+        with pytest.raises(ValueError):
+            be.device_status()
+        be.check(be.lib().nntr_cuda_clear_device_status())
+
+    be.paged_attention(c.q, c.k, c.v, table, start, context, new)
+    told()
+    be.paged_append(qkv[:, :512], qkv[:, 512:640], qkv[:, 640:], c.k, c.v, table, start, context, new, cos, sin)
+    told()

@@ -385,11 +385,13 @@ int nntr_cuda_paged_append_dev(const nntr_paged_cache *c, const nntr_paged_batch
                                unsigned flags, void *stream);
 /** Attention of the new tokens over the pages (their own rows are in them already). The query at position p sees the rows
  *  j <= p with j > p - window (UINT_MAX: all) or j < first_tokens; scores are scaled by 1 / sqrt(head_dim); sink: device fp32 [n_heads_q]
- *  logits that join the softmax without a value, or NULL. A query that sees nothing gets zeros. Cache rows that no query of a sequence sees may
- *  hold anything; the rows that one of them sees are expected to be finite (a score that is no number or +inf makes that query's result NaN). q: rows of the caches' type; out: of the same type
+ *  logits that join the softmax without a value, or NULL. A query that sees nothing gets zeros. Cache rows that no query of a sequence sees
+ *  may hold anything, and pages with such rows alone need not be there (-1 in the page table); the rows that one of them sees are expected to
+ *  be finite (a score that is no number or +inf makes that query's result NaN). q: rows of the caches' type; out: of the same type
  *  or fp32 (out_dtype NNTR_F32); both 16-byte aligned, ld_q and ld_out multiples of 8. Scores, sums and accumulators are fp32,
  *  probabilities are rounded to the caches' type before they meet the values: the difference from exact arithmetic is about one
- *  rounding to that type (also of fp32 results). No workspace. Not bit-compatible with nntr_cuda_attention_step_dev. */
+ *  rounding to that type (also of fp32 results). No workspace. Not bit-compatible with nntr_cuda_attention_step_dev, nor with another
+ *  batch, max_new or max_rows, which choose how sums are split. */
 int nntr_cuda_paged_attention_dev(const nntr_paged_cache *c, const nntr_paged_batch *b, const void *q, int64_t ld_q,
                                   unsigned window, unsigned first_tokens, const float *sink, void *out, int out_dtype,
                                   int64_t ld_out, unsigned flags, void *stream);

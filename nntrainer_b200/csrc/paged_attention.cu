@@ -41,7 +41,8 @@ int read_paged_attn_status(int *out, bool clear) {
  * warps of a CTA join through shared memory, the CTAs of a cluster, which share the cache rows of one (sequence, kv head, tile),
  * through each other's.
  * Bandwidth bounds it: 2 * 2 * head_dim bytes per cache row and kv head. 64 streams of 150 to 8192 rows, 8 kv heads of 128: 172 us, 6444
- * GB/s, 0.99 of a copy's rate; 64 of 8192 rows 304 us, 7071 GB/s. One of 500 rows: 6.4 us, launch, first loads and join. */
+ * GB/s, 0.99 of a copy's rate; 64 of 8192 rows 304 us, 7071 GB/s. One of 500 rows: 6.2 us, launch, first loads and join. Drafts, 16 x 5 tokens
+ * of 32 heads on 8 at 2000 rows: 32 us where the bytes take 20 (two tiles read the same rows, the second time from L2); 16 x 9 by the other kernel 36. */
 constexpr int PD_KEYS = 16; // of a block: no more than the smallest page
 constexpr uint32_t PD_POLLS = 1u << 22;
 template <int HD, int W> struct PdCfg { // W warps

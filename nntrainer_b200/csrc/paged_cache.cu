@@ -88,9 +88,9 @@ template <typename T> __device__ __forceinline__ void store4(T *p, const float4 
  * heads whose loads are on their way together, before it is looked up where the token belongs. Many tokens are bound by bandwidth, if only
  * few instructions go into an element: what a head's lanes need to know of it is computed once, mean and root by a multiplication and the
  * approximate reciprocal root (2^-22). VEC: rows, gammas and tables are 16-byte aligned.
- * 3760 tokens of 32 + 2 x 8 heads of 128 (139 MB beside the tables): 31.5 us, 4.4 TB/s; one head a lane group, CTAs by heads and
+ * 3760 tokens of 32 + 2 x 8 heads of 128 (139 MB beside the tables): 30.3 us, 4.6 TB/s; one head a lane group, CTAs by heads and
  * divisions 36.2. What is left is waiting: a lane group asks for a token's rows when it is through with the one in front (issue slots 63 %, HBM
- * 44 %). 64 tokens: 3.3 us, the latency of a launch, of one head's loads and of its sum. */
+ * 45 %). 64 tokens: 3.3 us, the latency of a launch, of one head's loads and of its sum. */
 template <typename T, int U, bool VEC>
 __global__ void __launch_bounds__(PA_THREADS, U == 1 ? 5 : 4) paged_append_kernel(AppendArgs a, PagedGeom g, PagedBatch s) {
   pdl_launch_dependents();

@@ -18,8 +18,12 @@
  * equal logits, top_k and top_p both far down) the whole cluster goes by digits over the whole row.
  *
  * What bounds it: for a row the chain of passes (greatest logit, histogram, list, cuts, draw: five to eight barriers of the cluster or CTA
- * each), one row of 151936 logits 13.9 us; for many rows the FMA pipes in the second reading (17 operations a logit), 128 rows of 201088 (103 MB) 54 us,
- * 1.9 TB/s. All weights in double precision and digits over the whole row: 1240 and 2234 us.
+ * each), one row of 151936 logits with top_k 20 and top_p 0.95 14.0 us. Many rows: 128 of 201088 (103 MB) with top_p 0.9 and min_p 0.02 53 us, 1.9 TB/s, wait for
+ * the loads of pass after pass (five of thirteen clocks between two instructions of a warp). No unit is the bound: issue slots 45 %, ALU
+ * 25, FMA pipes 21. Half of the second reading comes from HBM once more, and 256 CTAs leave 40 of the 148 SMs with one in place of two (75000
+ * clocks at work against 126000). As first built, all weights in double precision and digits over the whole row: 1240 and 2234 us.
+ * Digits over the whole row as they are now, for 1 and 128 rows: top_k 20000 with top_p 0.9 161 and 964 us; temperature 1e-5 (below |greatest logit| / 7e5,
+ * where weights are double precision throughout) 30 and 168, 24 at temperature 1; equal logits 29 and 132; top_p 0.9 of flat rows 170 and 747.
  */
 #include "cluster.cuh"
 #include "pipeline.cuh"

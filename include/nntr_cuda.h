@@ -390,7 +390,8 @@ int nntr_cuda_paged_append_dev(const nntr_paged_cache *c, const nntr_paged_batch
  *  be finite (a score that is no number or +inf makes that query's result NaN). q: rows of the caches' type; out: of the same type
  *  or fp32 (out_dtype NNTR_F32); both 16-byte aligned, ld_q and ld_out multiples of 8. Scores, sums and accumulators are fp32,
  *  probabilities are rounded to the caches' type before they meet the values: the difference from exact arithmetic is about one
- *  rounding to that type (also of fp32 results). No workspace. Not bit-compatible with nntr_cuda_attention_step_dev, nor with another
+ *  rounding to that type (also of fp32 results). In contexts beyond some 2^19 rows the tensor cores' accumulators, which cut off what lies
+ *  below their 24 bits, add to that: where values have one sign up to rows * 2^-30 of them for chunks, rows * 2^-34 for few rows. No workspace. Not bit-compatible with nntr_cuda_attention_step_dev, nor with another
  *  batch, max_new or max_rows, which choose how sums are split. */
 int nntr_cuda_paged_attention_dev(const nntr_paged_cache *c, const nntr_paged_batch *b, const void *q, int64_t ld_q,
                                   unsigned window, unsigned first_tokens, const float *sink, void *out, int out_dtype,

@@ -103,3 +103,21 @@ def test_as_many_rows_as_there_may_be(be):
         assert slack < 1e-6 or int(idx[r]) == i
     with pytest.raises(NotImplementedError):
         be.sample(torch.zeros(65536, 2, device="cuda"), torch.zeros(65536, device="cuda"))
+
+
+@pytest.mark.parametrize("heads,new,ctx", [((4096, 1, 8), [1], [20]), ((4096, 512, 64), [3], [40]), ((4096, 1, 128), [2, 1], [30, 9])])
+def test_as_many_heads_as_there_may_be(be, heads, new, ctx):
+    c = Case(new, ctx, heads, F16, 16, seed=95)
+    c.check(c.attend(be))
+
+
+@pytest.mark.parametrize("new", [1, 9])
+def test_as_many_sequences_as_there_may_be(be, new):
+    """Three sequences, 21845 times: all give what three alone give."""
+    c = Case([new] * 3, [new + 4, new, new + 8], (8, 1, 64), BF16, 16, seed=96)
+    start = torch.arange(65536, dtype=torch.int32, device="cuda") * new
+    out = be.paged_attention(c.q.repeat(21845, 1, 1), c.k, c.v, c.table.repeat(21845, 1), start, c.context.repeat(21845), new, new + 8)
+    out = out.view(21845, 3 * new, 8, 64)
+    c.check(out[0])
+    assert bool((out == out[0]).all())
+    be.device_status()

@@ -149,8 +149,9 @@ __device__ __forceinline__ float fma_sat(float a, float b, float c) { // a b + c
 
 /* 32 scores of a row to probabilities 2^x, x = s * scale - base, packed, and their sum. Some of the pairs are computed on the FMA pipes
  * beside the special function unit, which alone would take as many clocks as a step's products: (UPTO - x) / (UPTO - FROM) cut to 0 .. 1
- * (a power of two: nothing is rounded on the way back), x = n + f with f in [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f by the
- * polynomial of the least greatest relative error with value 1 at 0 (fp16: fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent.
+ * (a power of two: nothing is rounded on the way back; the cut value is to 2^-25, x to 2^-19, in bf16 2^-18), x = n + f with f in
+ * [-1/2, 1/2] (the low bits of x + 1.5 * 2^23 are n), 2^f by the polynomial of the least greatest relative error with value 1 at 0 (fp16:
+ * fourth degree, 2^-18.4; bf16: third, 2^-13.2), n into the exponent.
  * The cut is what keeps n inside it: in a step that goes by an older maximum x may be anything. It costs nothing where clamping x from below and
  * above took 2.4 % of the long chunks' time and a vote on the greatest x 5 %. What is masked is -inf: zero at FROM, also in bf16 (2^-127
  * has the exponent 0 and no mantissa). */
